@@ -13,7 +13,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liba11spec.so")
 
 OK, EINVAL, EBOUNDS, ECUDA, ETIMEOUT, ENONFINITE, ENOSPACE, EUNSUPPORTED = range(8)
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
+ACT_NONE, ACT_SILU, ACT_GELU = 0, 1, 2
+NORM_MAX_DIM = 16384
 GREEDY, STOCH_ONEHOT, STOCH_DRAFT = 0, 1, 2
 PAGE_TOKENS = 16
 NGRAM_MAX_UPDATES = 8192
@@ -73,10 +75,18 @@ def _load() -> C.CDLL:
     lib.a11s_lm_head.argtypes = [vp, vp, i32, i32, i32, f32, vp, i64, vp, vp, sz, vp]
     lib.a11s_accept_recorded.argtypes = [i32, vp, i64, f32, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp,
                                          vp, vp, vp, sz, vp]
+    lib.a11s_add_rms_norm.argtypes = [i32, vp, i64, vp, i64, vp, i32, i32, f32, vp, i64, i32, vp, i64, vp, vp]
+    lib.a11s_linear.argtypes = [i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, i64, vp, i64,
+                                vp, sz, vp]
+    lib.a11s_chunk_attention_workspace_bytes.restype = sz
+    lib.a11s_chunk_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32]
+    lib.a11s_chunk_attention.argtypes = [vp, i64, vp, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, f32,
+                                         vp, vp, vp, sz, vp]
     for name in ("a11s_read_status", "a11s_accept", "a11s_tree_attention", "a11s_kv_compact",
                  "a11s_ngram_expand", "a11s_verify_chain", "a11s_accept_static", "a11s_kv_pool_init",
                  "a11s_kv_reserve", "a11s_kv_release", "a11s_kv_free_sequences", "a11s_ngram_update",
-                 "a11s_next_roots", "a11s_lm_head", "a11s_accept_recorded"):
+                 "a11s_next_roots", "a11s_lm_head", "a11s_accept_recorded", "a11s_add_rms_norm", "a11s_linear",
+                 "a11s_chunk_attention"):
         getattr(lib, name).restype = C.c_int
     if lib.a11s_abi_version() != 1:
         raise ImportError("liba11spec.so ABI version mismatch")
@@ -98,4 +108,5 @@ def symbols():
             "a11s_tree_attention_workspace_bytes", "a11s_tree_attention", "a11s_kv_compact",
             "a11s_ngram_expand", "a11s_ngram_bucket", "a11s_verify_chain", "a11s_kv_pool_init",
             "a11s_kv_reserve", "a11s_kv_release", "a11s_kv_free_sequences", "a11s_ngram_update",
-            "a11s_next_roots", "a11s_lm_head_keys_bytes", "a11s_lm_head", "a11s_accept_recorded"]
+            "a11s_next_roots", "a11s_lm_head_keys_bytes", "a11s_lm_head", "a11s_accept_recorded",
+            "a11s_add_rms_norm", "a11s_linear", "a11s_chunk_attention_workspace_bytes", "a11s_chunk_attention"]

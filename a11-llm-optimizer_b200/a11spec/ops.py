@@ -7,6 +7,7 @@ torch's caching allocator unless the caller passes one.
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -217,6 +218,215 @@ def lm_head(hidden: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tens
     if check_status:
         raise_on_status(ws)
     return out, keys, ws
+
+
+# --------------------------------------------------------------------------- K8, K9, K10
+def _rows(t: torch.Tensor, name: str, dim: int, dtype, device):
+    """Element stride between the rows of t [..., dim]: unit column stride, rows evenly spaced."""
+    if not t.is_cuda or t.device != device:
+        raise A11Error(_lib.EINVAL, f"{name} must be on {device}")
+    if t.dtype != dtype:
+        raise A11Error(_lib.EINVAL, f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() == 0 or t.shape[-1] != dim:
+        raise A11Error(_lib.EINVAL, f"{name} must be [..., {dim}], got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return dim
+    if t.dim() == 1:
+        raise A11Error(_lib.EINVAL, f"{name} must have unit column stride")
+    if t.numel() == 0:
+        return dim
+    if t.stride(-1) != 1 and dim > 1:
+        raise A11Error(_lib.EINVAL, f"{name} must have unit column stride")
+    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]  # an axis of one row has no stride
+    for (_, s), (n, inner) in zip(lead, lead[1:]):
+        if s != inner * n:
+            raise A11Error(_lib.EINVAL, f"{name} rows must be evenly spaced")
+    return lead[-1][1] if lead else dim
+
+
+def _vector(t: Optional[torch.Tensor], name: str, n: int, dtype, device):
+    """Pointer of a dense vector of n elements (None: null)."""
+    if t is None:
+        return None
+    if not t.is_cuda or t.device != device or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise A11Error(_lib.EINVAL, f"{name} must be {n} contiguous {dtype} elements on {device}")
+    return t.data_ptr()
+
+
+def _on_its_device(op):
+    """Runs `op` with the device of its first tensor current (its stream is that device's current one)."""
+    @functools.wraps(op)
+    def call(first: torch.Tensor, *args, **kw):
+        if not first.is_cuda:
+            raise A11Error(_lib.EINVAL, f"{op.__name__}: CUDA tensors expected")
+        if first.device.index == torch.cuda.current_device():
+            return op(first, *args, **kw)
+        with torch.cuda.device(first.device):
+            return op(first, *args, **kw)
+    return call
+
+
+@_on_its_device
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
+                 scales: Optional[torch.Tensor] = None, sum_out: Optional[torch.Tensor] = None):
+    """K8. h = x + residual and y = h * rsqrt(mean(h^2) + eps) * weight per row of
+    x [..., dim] (bf16 or fp32; residual and weight [dim] of the same type).
+
+    Returns (y, scales, h). y has out_dtype (default: out's type, else x's): x's
+    type, or torch.float8_e4m3fn with `scales` fp32 [...], one per row (y stands
+    for out * scale). h is x + residual rounded to x's type (sum_out when given,
+    which may be x or residual itself: in place); None without a residual.
+    Tensors may be views whose rows are evenly spaced."""
+    dev, dim = x.device, x.shape[-1] if x.dim() else 0
+    code = _NORM_TYPES.get(x.dtype)
+    if code is None or dim == 0:
+        raise A11Error(_lib.EINVAL, f"add_rms_norm: x must be float32 or bfloat16 [..., dim], got {x.dtype} {tuple(x.shape)}")
+    rows = x.numel() // dim
+    xs = _rows(x, "x", dim, x.dtype, dev)
+    wp = _vector(weight, "weight", dim, x.dtype, dev)
+    if out is None:
+        out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=dev)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise A11Error(_lib.EINVAL, f"add_rms_norm: out is {out.dtype}, out_dtype {out_dtype}")
+    e4m3 = out.dtype == torch.float8_e4m3fn
+    os_ = _rows(out, "out", dim, torch.float8_e4m3fn if e4m3 else x.dtype, dev)
+    if e4m3 and scales is None:
+        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    elif scales is not None and not e4m3:
+        raise A11Error(_lib.EINVAL, "add_rms_norm: scales go with e4m3 output")
+    sp = _vector(scales, "scales", rows, torch.float32, dev)
+    rp = hp = None
+    rs = hs = 0
+    if residual is not None:
+        rs, rp = _rows(residual, "residual", dim, x.dtype, dev), residual.data_ptr()
+        if sum_out is None:
+            sum_out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        hs, hp = _rows(sum_out, "sum_out", dim, x.dtype, dev), sum_out.data_ptr()
+    elif sum_out is not None:
+        raise A11Error(_lib.EINVAL, "add_rms_norm: sum_out without a residual")
+    if out.numel() != x.numel() or any(t is not None and t.numel() != x.numel() for t in (residual, sum_out)):
+        raise A11Error(_lib.EINVAL, "add_rms_norm: x, residual, sum_out and out must have the same rows")
+    check(lib.a11s_add_rms_norm(code, x.data_ptr(), xs, rp, rs, wp, rows, dim, eps, hp, hs,
+                                _lib.E4M3 if e4m3 else code, out.data_ptr(), os_, sp, _stream()))
+    return out, scales, sum_out
+
+
+_NORM_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_LINEAR_TYPES = {torch.bfloat16: _lib.BF16, torch.float8_e4m3fn: _lib.E4M3}
+_ACTIVATIONS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
+
+
+@_on_its_device
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           activation: Optional[str] = None, gate: Optional[torch.Tensor] = None,
+           gate_bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+           x_scale: Optional[torch.Tensor] = None, weight_scale: Optional[torch.Tensor] = None,
+           gate_scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+           ws: Optional[torch.Tensor] = None, check_status: bool = False) -> torch.Tensor:
+    """K9. x [..., K], weight [N, K] -> act(x weight^T + bias) + residual, or with
+    a gate [N, K]: act(x gate^T + gate_bias) * (x weight^T + bias) + residual;
+    bf16 [..., N], the sums and the epilogue in fp32.
+
+    x, weight and gate are bf16, or all e4m3 with fp32 scales per row of x
+    (x_scale [...]) and of the weights (weight_scale, gate_scale [N]): what
+    add_rms_norm(out_dtype=torch.float8_e4m3fn) gives. activation: None, "silu"
+    or "gelu" (erf). x, out and residual may be views whose rows are evenly
+    spaced (x: 16-byte multiples); out may be residual itself. ws (256 bytes)
+    receives the status word; check_status=True reads it (and synchronises)."""
+    dev = x.device
+    if weight.dim() != 2 or x.dim() == 0:
+        raise A11Error(_lib.EINVAL, "linear: x [..., K] and weight [N, K] expected")
+    N, K = weight.shape
+    code = _LINEAR_TYPES.get(x.dtype)
+    if code is None:
+        raise A11Error(_lib.EINVAL, f"linear: x must be bfloat16 or float8_e4m3fn, got {x.dtype}")
+    if activation not in _ACTIVATIONS:
+        raise A11Error(_lib.EINVAL, f"linear: activation {activation!r}, not None, 'silu' or 'gelu'")
+    rows = x.numel() // K if K else 0
+    xs = _rows(x, "x", K, x.dtype, dev)
+    wp = _vector(weight, "weight", N * K, x.dtype, dev)
+    if gate is not None and gate.shape != weight.shape:
+        raise A11Error(_lib.EINVAL, f"linear: gate {tuple(gate.shape)} differs from weight {tuple(weight.shape)}")
+    gp = _vector(gate, "gate", N * K, x.dtype, dev)
+    if out is None:
+        out = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=dev)
+    os_ = _rows(out, "out", N, torch.bfloat16, dev)
+    rs, rp = 0, None
+    if residual is not None:
+        rs, rp = _rows(residual, "residual", N, torch.bfloat16, dev), residual.data_ptr()
+    if out.numel() != rows * N or (residual is not None and residual.numel() != rows * N):
+        raise A11Error(_lib.EINVAL, f"linear: out and residual must have x's {rows} rows")
+    if ws is None and check_status:
+        ws = workspace(256, dev)
+    check(lib.a11s_linear(code, x.data_ptr(), xs, _vector(x_scale, "x_scale", rows, torch.float32, dev), wp,
+                          _vector(weight_scale, "weight_scale", N, torch.float32, dev), gp,
+                          _vector(gate_scale, "gate_scale", N, torch.float32, dev),
+                          _vector(bias, "bias", N, torch.bfloat16, dev),
+                          _vector(gate_bias, "gate_bias", N, torch.bfloat16, dev), rows, K, N,
+                          _ACTIVATIONS[activation], rp, rs, out.data_ptr(), os_, _ptr(ws),
+                          0 if ws is None else ws.numel(), _stream()))
+    if check_status:
+        raise_on_status(ws)
+    return out
+
+
+def chunk_attention_workspace_bytes(batch, max_new, num_q_heads, num_kv_heads, head_dim, max_kv_len):
+    return int(lib.a11s_chunk_attention_workspace_bytes(batch, max_new, num_q_heads, num_kv_heads, head_dim,
+                                                        max_kv_len))
+
+
+@_on_its_device
+def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
+                    ctx_lens: torch.Tensor, n_new: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    max_kv_len: Optional[int] = None, want_lse: bool = False, out: Optional[torch.Tensor] = None,
+                    lse: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None,
+                    check_status: bool = False):
+    """K10. q [B, n, Hq, D] bf16 (D 64 or 128; tokens may be apart, as in a slice
+    of a fused projection's rows): new tokens of each sequence, whose
+    K/V already sit in the pools [P, 16, Hkv, D] at positions ctx_lens[b] + i of
+    page_table [B, maxpages]. Token i < n_new[b] (default n) sees positions
+    0 .. ctx_lens[b] + i; the other rows come back as zeros. max_kv_len: an upper
+    bound of ctx_lens[b] + n_new[b] (default: what the page table holds).
+    Returns (out, lse, ws); lse [B, n, Hq] fp32 with want_lse, else None. Pass ws
+    again to reuse it; calls that overlap on the GPU need one each."""
+    if q.dim() != 4 or k_pool.dim() != 4:
+        raise A11Error(_lib.EINVAL, "chunk_attention: q [B, n, Hq, D] and pools [P, 16, Hkv, D] expected")
+    B, N, Hq, D = q.shape
+    P, pg, Hkv, D2 = k_pool.shape
+    if pg != _lib.PAGE_TOKENS or D2 != D or v_pool.shape != k_pool.shape:
+        raise A11Error(_lib.EINVAL, "pool shape must be [P, 16, Hkv, D] for K and V")
+    dev = q.device
+    if q.dtype != torch.bfloat16 or (D > 1 and q.stride(3) != 1) or (Hq > 1 and q.stride(2) != D):
+        raise A11Error(_lib.EINVAL, "q must be bfloat16 with a token's heads dense")
+    qs = q.stride(1) if N > 1 else q.stride(0) if B > 1 else Hq * D
+    if B > 1 and q.stride(0) != N * qs:
+        raise A11Error(_lib.EINVAL, "q tokens must be evenly spaced")
+    kp = _vector(k_pool, "k_pool", k_pool.numel(), torch.bfloat16, dev)
+    vp = _vector(v_pool, "v_pool", k_pool.numel(), torch.bfloat16, dev)
+    if page_table.dim() != 2 or page_table.shape[0] != B:
+        raise A11Error(_lib.EINVAL, f"page_table must be [{B}, maxpages], got {tuple(page_table.shape)}")
+    pages = page_table.shape[1]
+    tp = _vector(page_table, "page_table", B * pages, torch.int32, dev)
+    cp = _vector(ctx_lens, "ctx_lens", B, torch.int32, dev)
+    np_ = _vector(n_new, "n_new", B, torch.int32, dev)
+    if max_kv_len is None:
+        max_kv_len = pages * _lib.PAGE_TOKENS
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    op = _vector(out, "out", q.numel(), torch.bfloat16, dev)
+    if want_lse and lse is None:
+        lse = torch.empty(B, N, Hq, dtype=torch.float32, device=dev)
+    lp = _vector(lse, "lse", B * N * Hq, torch.float32, dev)
+    if ws is None:
+        ws = workspace(chunk_attention_workspace_bytes(B, N, Hq, Hkv, D, max_kv_len), dev)
+    check(lib.a11s_chunk_attention(q.data_ptr(), qs, kp, vp, P, tp, pages, cp, np_, B, N, Hq, Hkv, D, max_kv_len, scale, op, lp,
+                                   ws.data_ptr(), ws.numel(), _stream()))
+    if check_status:
+        raise_on_status(ws)
+    return out, lse, ws
 
 
 # --------------------------------------------------------------------------- K4

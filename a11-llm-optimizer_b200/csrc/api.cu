@@ -579,4 +579,177 @@ int a11s_tree_attention(const void *q, const void *k_pool, const void *v_pool, i
     return A11S_OK;
 }
 
+// ------------------------------------------------------------------- K10
+size_t a11s_chunk_attention_workspace_bytes(int32_t batch, int32_t max_new, int32_t num_q_heads,
+                                            int32_t num_kv_heads, int32_t head_dim, int32_t max_kv_len) {
+    if (batch < 0 || max_new < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || num_q_heads / num_kv_heads > 128 ||
+        head_dim < 1 || max_kv_len < 1)
+        return 0;
+    const a11s::ChunkPlan plan = a11s::chunk_attention_plan(batch, max_new, num_q_heads, num_kv_heads, max_kv_len);
+    return kHeaderBytes + up256(a11s::chunk_attention_partials_bytes(batch, max_new, num_q_heads, head_dim, plan.splits));
+}
+
+int a11s_chunk_attention(const void *q, int64_t q_stride, const void *k_pool, const void *v_pool, int32_t num_pages,
+                         const int32_t *page_table, int32_t max_pages_per_seq, const int32_t *ctx_lens,
+                         const int32_t *n_new, int32_t batch, int32_t max_new, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t max_kv_len, float scale, void *out,
+                         float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+    if (head_dim != 64 && head_dim != 128)
+        return fail(A11S_EUNSUPPORTED, "a11s_chunk_attention: head_dim %d is neither 64 nor 128", head_dim);
+    if (batch < 0 || max_new < 1 || num_kv_heads < 1 || num_q_heads < 1 || num_pages < 1 || max_pages_per_seq < 1 ||
+        max_kv_len < 1)
+        return fail(A11S_EINVAL, "a11s_chunk_attention: non-positive size");
+    if (num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > 128)
+        return fail(A11S_EUNSUPPORTED, "a11s_chunk_attention: %d query heads on %d KV heads (a multiple, at most 128 each)",
+                    num_q_heads, num_kv_heads);
+    if ((int64_t)max_pages_per_seq * A11S_PAGE_TOKENS < max_kv_len)
+        return fail(A11S_EINVAL, "a11s_chunk_attention: page table shorter than max_kv_len");
+    if (q_stride < (int64_t)num_q_heads * head_dim || q_stride % 8)
+        return fail(A11S_EINVAL, "a11s_chunk_attention: q_stride %lld is less than a token's heads or no multiple of 8",
+                    (long long)q_stride);
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(A11S_EINVAL, "a11s_chunk_attention: bad scale");
+    if (batch == 0) return empty_batch_status(workspace, workspace_bytes, stream, "a11s_chunk_attention: clearing status");
+    if (!q || !k_pool || !v_pool || !page_table || !ctx_lens || !out || !workspace)
+        return fail(A11S_EINVAL, "a11s_chunk_attention: null required pointer");
+    if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || !aligned16(workspace))
+        return fail(A11S_EINVAL, "a11s_chunk_attention: tensors must be 16-byte aligned");
+    a11s::ChunkAttnArgs a{};
+    a.plan = a11s::chunk_attention_plan(batch, max_new, num_q_heads, num_kv_heads, max_kv_len);
+    const size_t need = kHeaderBytes + up256(a11s::chunk_attention_partials_bytes(batch, max_new, num_q_heads, head_dim,
+                                                                                  a.plan.splits));
+    if (workspace_bytes < need)
+        return fail(A11S_ENOSPACE, "a11s_chunk_attention: workspace %zu < %zu bytes", workspace_bytes, need);
+    if ((double)a.plan.ctiles * batch * a.plan.splits * num_kv_heads > 2147483647.0 ||
+        (double)batch * max_new * num_q_heads > 2147483647.0)
+        return fail(A11S_EUNSUPPORTED, "a11s_chunk_attention: more rows than a launch holds");
+    a.q = q;
+    a.q_stride = q_stride;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.num_pages = num_pages;
+    a.page_table = page_table;
+    a.max_pages = max_pages_per_seq;
+    a.ctx_lens = ctx_lens;
+    a.n_new = n_new;
+    a.B = batch;
+    a.N = max_new;
+    a.Hq = num_q_heads;
+    a.Hkv = num_kv_heads;
+    a.D = head_dim;
+    a.scale = scale;
+    a.out = out;
+    a.lse = lse;
+    char *ws = static_cast<char *>(workspace);
+    a.status = reinterpret_cast<a11s::StatusWord *>(ws);
+    a.part_o = reinterpret_cast<float *>(ws + kHeaderBytes);
+    a.part_ml = a.part_o + (size_t)a.plan.splits * batch * max_new * num_q_heads * head_dim;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(a11s::StatusWord), s);
+    if (e != cudaSuccess) return cuda_fail(e, "a11s_chunk_attention: clearing status");
+    e = a11s::launch_chunk_attention(a, s);
+    if (e != cudaSuccess) return cuda_fail(e, "a11s_chunk_attention: launch");
+    return A11S_OK;
+}
+
+// ------------------------------------------------------------------- K8
+int a11s_add_rms_norm(int32_t dtype, const void *x, int64_t x_stride, const void *residual,
+                      int64_t residual_stride, const void *weight, int32_t rows, int32_t dim, float eps,
+                      void *sum, int64_t sum_stride, int32_t out_dtype, void *out, int64_t out_stride,
+                      float *scales, void *stream) {
+    if (dtype != A11S_F32 && dtype != A11S_BF16) return fail(A11S_EINVAL, "a11s_add_rms_norm: dtype %d", dtype);
+    if (out_dtype != dtype && out_dtype != A11S_E4M3)
+        return fail(A11S_EINVAL, "a11s_add_rms_norm: out_dtype %d is neither the input's nor e4m3", out_dtype);
+    if (rows < 0 || dim < 1) return fail(A11S_EINVAL, "a11s_add_rms_norm: bad sizes");
+    if (dim > A11S_NORM_MAX_DIM)
+        return fail(A11S_EUNSUPPORTED, "a11s_add_rms_norm: dim %d > %d", dim, A11S_NORM_MAX_DIM);
+    if (x_stride < dim || out_stride < dim || (residual && residual_stride < dim) || (sum && sum_stride < dim))
+        return fail(A11S_EINVAL, "a11s_add_rms_norm: a row stride is smaller than dim %d", dim);
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(A11S_EINVAL, "a11s_add_rms_norm: bad eps");
+    if (rows == 0) return A11S_OK;
+    if (!x || !weight || !out) return fail(A11S_EINVAL, "a11s_add_rms_norm: null required pointer");
+    if ((out_dtype == A11S_E4M3) != (scales != nullptr))
+        return fail(A11S_EINVAL, "a11s_add_rms_norm: scales go with e4m3 output and only with it");
+    const uintptr_t mis = dtype == A11S_BF16 ? 1 : 3;
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(weight) |
+          reinterpret_cast<uintptr_t>(sum)) & mis) || (out_dtype != A11S_E4M3 && (reinterpret_cast<uintptr_t>(out) & mis)) ||
+        (reinterpret_cast<uintptr_t>(scales) & 3))
+        return fail(A11S_EINVAL, "a11s_add_rms_norm: a tensor is not aligned to its elements");
+    a11s::NormArgs a{};
+    a.x = x;
+    a.residual = residual;
+    a.weight = weight;
+    a.sum = sum;
+    a.out = out;
+    a.scales = scales;
+    a.x_stride = x_stride;
+    a.res_stride = residual ? residual_stride : 0;
+    a.sum_stride = sum ? sum_stride : 0;
+    a.out_stride = out_stride;
+    a.rows = rows;
+    a.dim = dim;
+    a.eps = eps;
+    a.bf16 = dtype == A11S_BF16;
+    a.e4m3 = out_dtype == A11S_E4M3;
+    const cudaError_t e = a11s::launch_add_rms_norm(a, reinterpret_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "a11s_add_rms_norm: launch");
+    return A11S_OK;
+}
+
+// ------------------------------------------------------------------- K9
+int a11s_linear(int32_t dtype, const void *x, int64_t x_stride, const float *x_scale, const void *weight,
+                const float *weight_scale, const void *gate, const float *gate_scale, const void *bias,
+                const void *gate_bias, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t activation,
+                const void *residual, int64_t residual_stride, void *out, int64_t out_stride,
+                void *workspace, size_t workspace_bytes, void *stream) {
+    if (dtype != A11S_BF16 && dtype != A11S_E4M3) return fail(A11S_EINVAL, "a11s_linear: dtype %d", dtype);
+    const int per16 = dtype == A11S_E4M3 ? 16 : 8;
+    if (rows < 0 || in_dim < 1 || out_dim < 1) return fail(A11S_EINVAL, "a11s_linear: bad sizes");
+    if (in_dim % per16 || x_stride % per16)
+        return fail(A11S_EINVAL, "a11s_linear: in_dim and x_stride must be multiples of %d (16 bytes)", per16);
+    if (x_stride < in_dim || out_stride < out_dim || (residual && residual_stride < out_dim))
+        return fail(A11S_EINVAL, "a11s_linear: a row stride is smaller than its row");
+    if (activation < A11S_ACT_NONE || activation > A11S_ACT_GELU)
+        return fail(A11S_EINVAL, "a11s_linear: activation %d", activation);
+    if (gate_bias && !gate) return fail(A11S_EINVAL, "a11s_linear: gate_bias without gate");
+    if (workspace && (workspace_bytes < 256 || !aligned16(workspace)))
+        return fail(A11S_ENOSPACE, "a11s_linear: workspace %zu < 256 bytes or not 16-byte aligned", workspace_bytes);
+    if (rows == 0) return empty_batch_status(workspace, workspace_bytes, stream, "a11s_linear: clearing status");
+    if (!x || !weight || !out) return fail(A11S_EINVAL, "a11s_linear: null required pointer");
+    const bool e4m3 = dtype == A11S_E4M3;
+    if (e4m3 != (x_scale != nullptr) || e4m3 != (weight_scale != nullptr) || (e4m3 && gate) != (gate_scale != nullptr))
+        return fail(A11S_EINVAL, "a11s_linear: scales go with e4m3 operands and only with them");
+    if (!aligned16(x) || !aligned16(weight) || !aligned16(gate))
+        return fail(A11S_EINVAL, "a11s_linear: x, weight and gate must be 16-byte aligned");
+    if (((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(gate_bias) | reinterpret_cast<uintptr_t>(residual) |
+          reinterpret_cast<uintptr_t>(out)) & 1) ||
+        ((reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(weight_scale) |
+          reinterpret_cast<uintptr_t>(gate_scale)) & 3))
+        return fail(A11S_EINVAL, "a11s_linear: a tensor is not aligned to its elements");
+    if (((double)rows / 128 + 1) * ((double)out_dim / 32 + 1) * 8 > 2147483647.0)
+        return fail(A11S_EUNSUPPORTED, "a11s_linear: more tiles than a launch holds");
+    a11s::LinearArgs a{};
+    a.x = x;
+    a.x_scale = x_scale;
+    a.weight = weight;
+    a.gate = gate;
+    a.w_scale = weight_scale;
+    a.g_scale = gate_scale;
+    a.bias = bias;
+    a.g_bias = gate_bias;
+    a.residual = residual;
+    a.out = out;
+    a.x_stride = x_stride;
+    a.res_stride = residual_stride;
+    a.out_stride = out_stride;
+    a.rows = rows;
+    a.K = in_dim;
+    a.N = out_dim;
+    a.act = activation;
+    a.e4m3 = e4m3;
+    a.status = static_cast<a11s::StatusWord *>(workspace);
+    const cudaError_t e = a11s::launch_linear(a, reinterpret_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "a11s_linear: launch");
+    return A11S_OK;
+}
+
 }  // extern "C"

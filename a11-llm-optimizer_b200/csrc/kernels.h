@@ -164,6 +164,61 @@ struct AttnArgs {
 
 cudaError_t launch_tree_attention(const AttnArgs &a, cudaStream_t s);
 
+// How a11s_chunk_attention cuts its work: tokens of a Q tile, CTAs along the
+// chunk, and at most `splits` splits of `split_blocks` 128-key blocks along the cache.
+struct ChunkPlan {
+    int32_t tokens = 1, ctiles = 1, splits = 1, split_blocks = 1;
+};
+ChunkPlan chunk_attention_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t max_kv_len);
+size_t chunk_attention_partials_bytes(int32_t B, int32_t N, int32_t Hq, int32_t D, int32_t splits);
+
+struct ChunkAttnArgs {
+    const void *q, *k_pool, *v_pool;
+    int64_t q_stride;  // elements between tokens of q
+    int32_t num_pages;
+    const int32_t *page_table;
+    int32_t max_pages;
+    const int32_t *ctx_lens, *n_new;  // n_new: nullable
+    int32_t B, N, Hq, Hkv, D;
+    float scale;
+    void *out;
+    float *lse;               // nullable
+    float *part_o, *part_ml;  // [splits][B][N][Hq][D], [splits][B][N][Hq][2] (reference maximum in log2 units, sum)
+    ChunkPlan plan;
+    StatusWord *status;
+};
+cudaError_t launch_chunk_attention(const ChunkAttnArgs &a, cudaStream_t s);
+
+struct NormArgs {
+    const void *x, *residual, *weight;  // residual: nullable
+    void *sum, *out;                    // sum: nullable
+    float *scales;                      // [rows] (e4m3 output) or null
+    int64_t x_stride, res_stride, sum_stride, out_stride;
+    int32_t rows, dim;
+    float eps;
+    bool bf16, e4m3;                    // input type (else fp32), output in e4m3 (else the input's type)
+};
+cudaError_t launch_add_rms_norm(const NormArgs &a, cudaStream_t s);
+
+struct LinearArgs {
+    const void *x;                // [rows][x_stride], bf16 or e4m3
+    const float *x_scale;         // [rows] (e4m3)
+    const void *weight, *gate;    // [N][K] of x's type; gate: nullable
+    const float *w_scale, *g_scale;  // [N] (e4m3)
+    const void *bias, *g_bias;    // bf16 [N], nullable
+    const void *residual;         // bf16 [rows][res_stride], nullable
+    void *out;                    // bf16 [rows][out_stride]
+    int64_t x_stride, res_stride, out_stride;
+    int32_t rows, K, N;
+    int32_t act;                  // A11S_ACT_*
+    bool e4m3;
+    StatusWord *status;           // nullable
+};
+cudaError_t launch_linear(const LinearArgs &a, cudaStream_t s);
+// rows at most kSkinnyRows: the weight-streaming kernel
+constexpr int kSkinnyRows = 32;
+cudaError_t launch_linear_skinny(const LinearArgs &a, cudaStream_t s);
+
 cudaError_t launch_verify_chain(const float *draft, const float *target, const float *uni, int B, int n,
                                 int32_t *accepted_len, int32_t *last_idx, StatusWord *st, cudaStream_t s);
 

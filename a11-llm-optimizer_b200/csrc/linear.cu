@@ -1,0 +1,669 @@
+// linear.cu - K9: matrix product with its epilogue on the tensor cores (TMA +
+// tcgen05, TMEM accumulators, sm_100a), bf16 or e4m3 operands.
+//
+//   v = (sum_k x[m][k] W[n][k]) sx[m] sw[n] + bias[n]
+//   u = (sum_k x[m][k] G[n][k]) sx[m] sg[n] + gate_bias[n]        (gated)
+//   y[m][n] = bf16_rn((gated ? act(u) v : act(v)) + residual[m][n])
+//
+// sums and everything after them in fp32, one rounding. The projections of the
+// reference's forward_layer (engine/pipeline.py:364-373, 403-405, 407-447:
+// torch.matmul, + bias, silu(gate) * up, h + ...). Semantics: include/a11spec.h
+// (a11s_linear).
+//
+// Three kernels, chosen in launch_linear by a cost model of their tiles:
+//   linear_skinny (linear_skinny.cu)  up to 32 rows: HBM-bound weight streaming
+//   linear_tile   128 rows x 64 or 128 weight rows a CTA, K split over the CTAs
+//                 of a cluster (1 to 8): sizes whose tiles alone would leave most
+//                 SMs idle. The partial sums meet in distributed shared memory,
+//                 added in rank order.
+//   linear_pair   persistent CTA pairs (cta_group::2), 256 x 256 tiles: sizes
+//                 that fill the GPU. Tensor-bound; structure as in lm_head.cu.
+// A gated product takes gate and weight rows side by side in one tile (half the
+// columns each), so x is staged once for both and act(u) v is formed from two
+// column ranges of one accumulator: the 2 N intermediate is never written.
+// Operand tiles are 128 bytes of K per row (64 bf16, 128 e4m3), 128-byte
+// swizzle: the types differ in the instruction and the tensor maps only.
+// Every mbarrier wait is bounded; a timeout sets ETIMEOUT, and the CTA drains
+// its copies and MMAs and returns.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "epilogue.cuh"
+#include "kernels.h"
+#include "tc_common.cuh"
+
+namespace a11s {
+
+namespace {
+constexpr int kThreads = 192;                    // TMA warp, MMA warp, 4 epilogue warps
+constexpr int kSliceBytes = 128;                 // bytes of K per row and slice
+constexpr long long kWaitBudget = 2000000000ll;  // ~1 s of SM clock
+
+struct LinParams {
+    const float *x_scale;
+    ColumnParams col;
+    const __nv_bfloat16 *residual;
+    __nv_bfloat16 *out;
+    int64_t res_stride, out_stride;
+    int32_t rows, N, act, m_tiles, n_tiles, slices, split;
+    int32_t tma_out, tma_res;  // linear_pair: out (and the residual) take tensor maps
+    StatusWord *status;
+};
+
+struct BarsCommon {
+    int32_t abort;
+    uint32_t tmem_base;
+};
+__device__ __forceinline__ bool aborted(BarsCommon *bs) { return *reinterpret_cast<volatile int32_t *>(&bs->abort) != 0; }
+__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, BarsCommon *bs, StatusWord *st) {
+    if (tc::mbar_wait(bar, parity, kWaitBudget)) return true;
+    *reinterpret_cast<volatile int32_t *>(&bs->abort) = 1;
+    report(st, A11S_ETIMEOUT, (int32_t)blockIdx.x);
+    return false;
+}
+// The status word is cleared by the launch's first thread: a report can only
+// follow a wait of about a second, long after every CTA of the launch started.
+__device__ __forceinline__ void clear_status(StatusWord *st) {
+    if (st && blockIdx.x == 0 && threadIdx.x == 0) *st = StatusWord{0, 0};
+}
+}  // namespace
+
+// ---------------------------------------------------------------------------- linear_tile
+namespace {
+constexpr int kTileM = 128;
+constexpr uint32_t kTileABytes = kTileM * kSliceBytes;  // 16 KB
+template <int BN>
+struct TileShape {
+    static constexpr uint32_t kStage = kTileABytes + BN * kSliceBytes;
+    static constexpr int kStages = BN == 64 ? 8 : 6;
+    static constexpr uint32_t kRing = kStages * kStage;  // 192 KB
+    static constexpr uint32_t kSmem = kRing + 512 + 1024;
+};
+struct TileBars : BarsCommon {
+    uint64_t full[8], empty[8], acc_full, drain;
+};
+static_assert(sizeof(TileBars) <= 512, "barrier block");
+}  // namespace
+
+// One 128 x BN tile (gated: 128 x BN/2 outputs) per cluster of p.split CTAs;
+// each CTA multiplies its share of the K slices.
+template <bool E4M3, bool GATED, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_tile(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
+                const __grid_constant__ CUtensorMap tg, const LinParams p) {
+    using S = TileShape<BN>;
+    constexpr int kOut = GATED ? BN / 2 : BN;  // output columns of a tile
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    TileBars *bs = reinterpret_cast<TileBars *>(sm + S::kRing);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % p.split, tile = blockIdx.x / p.split;  // clusters are consecutive CTAs
+    const int m0 = (tile % p.m_tiles) * kTileM, n0 = (tile / p.m_tiles) * kOut;
+    const int per = (p.slices + p.split - 1) / p.split;
+    const int s0 = min(rank * per, p.slices), ns = min(per, p.slices - s0);
+    clear_status(p.status);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) {
+            tc::mbar_init(&bs->full[s], 1);
+            tc::mbar_init(&bs->empty[s], 1);
+        }
+        tc::mbar_init(&bs->acc_full, 1);
+        tc::mbar_init(&bs->drain, 1);
+        bs->abort = 0;
+        tc::fence_barrier_init();
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(&bs->tmem_base, BN);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = bs->tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
+            for (int i = 0; i < ns; ++i) {
+                const int s = i % S::kStages, use = i / S::kStages;
+                if (use > 0 && !wait_or_abort(&bs->empty[s], (use - 1) & 1, bs, p.status)) break;
+                if (aborted(bs)) break;
+                uint8_t *a = sm + s * S::kStage;
+                const int k = (s0 + i) * kElems;
+                tc::mbar_arrive_expect_tx(&bs->full[s], S::kStage);
+                tc::tma_load_2d(a, &tx, &bs->full[s], k, m0);
+                if constexpr (GATED) {  // gate rows, then weight rows: kOut of each
+                    tc::tma_load_2d(a + kTileABytes, &tg, &bs->full[s], k, n0);
+                    tc::tma_load_2d(a + kTileABytes + kOut * kSliceBytes, &tw, &bs->full[s], k, n0);
+                } else {
+                    tc::tma_load_2d(a + kTileABytes, &tw, &bs->full[s], k, n0);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = E4M3 ? tc::idesc_e4m3_f32(kTileM, BN) : tc::idesc_bf16_f32(kTileM, BN, false);
+            bool ok = true;
+            for (int i = 0; i < ns && ok; ++i) {
+                const int s = i % S::kStages;
+                if (!(ok = wait_or_abort(&bs->full[s], (i / S::kStages) & 1, bs, p.status))) break;
+                tc::tc_fence_after();
+                const uint32_t a = tc::smem_u32(sm + s * S::kStage), b = a + kTileABytes;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    const uint64_t ad = tc::sdesc_sw128(a + kk * 32, 16, 1024), bd = tc::sdesc_sw128(b + kk * 32, 16, 1024);
+                    if constexpr (E4M3) tc::mma_e4m3_ss(tmem, ad, bd, idesc, (i | kk) != 0);
+                    else tc::mma_bf16_ss(tmem, ad, bd, idesc, (i | kk) != 0);
+                }
+                tc::mma_commit(&bs->empty[s]);
+            }
+            if (ok) tc::mma_commit(&bs->acc_full);
+            tc::mma_commit(&bs->drain);
+            tc::mbar_wait(&bs->drain, 0, kWaitBudget);
+        }
+        __syncwarp();
+    }
+    // ---------------- the accumulator is complete: the ring is free ----------------
+    // part: this CTA's sums, [BN][128] fp32, column-major (a warp's 32 rows are
+    // consecutive); stage: finished outputs of an epilogue warp, [32][cols + 1] fp32
+    float *part = reinterpret_cast<float *>(sm);
+    const int q = warp & 3, row = q * 32 + lane;  // of epilogue warps: TMEM lane = tile row
+    bool ok = true;
+    if (warp >= 2) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bs->acc_full, 0, bs, p.status));
+        if (ok) {
+            tc::tc_fence_after();
+            const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) {
+                float v[32];
+                if (ns > 0) {
+                    tc::tmem_ld32(tmem + lane_base + c, v);
+                } else {  // no K slice fell to this CTA
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) part[(c + e) * kTileM + row] = v[e];
+            }
+        }
+    }
+    tc::tc_fence_before();
+    tc::cluster_sync();  // every CTA's sums are in shared memory (and after a timeout nobody waits for them)
+    if (warp >= 2 && ok) {
+        const int cols = kOut / p.split, c0 = rank * cols;  // this CTA's output columns of the tile
+        float *stage = reinterpret_cast<float *>(sm + BN * kTileM * 4) + q * 32 * (kOut + 1);
+        const float xs = E4M3 && m0 + row < p.rows ? __ldg(p.x_scale + m0 + row) : 1.0f;
+        uint32_t src[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) src[r] = r < p.split ? tc::cluster_addr(part, r) : 0;
+        for (int c = 0; c < cols; ++c) {
+            // gated: the gate's columns are the first half of the tile
+            const uint32_t at = ((GATED ? kOut : 0) + c0 + c) * kTileM + row, gat = (c0 + c) * kTileM + row;
+            float v = 0.0f, u = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < p.split) {
+                    v += tc::ld_cluster_f32(src[r] + at * 4);
+                    if (GATED) u += tc::ld_cluster_f32(src[r] + gat * 4);
+                }
+            const int n = n0 + c0 + c;
+            if (n < p.N) v = finish<GATED>(v, u, xs, column<GATED>(p.col, n), p.act);
+            stage[lane * (cols + 1) + c] = v;
+        }
+        __syncwarp();
+        // rows of the warp, `cols` consecutive columns each, written coalesced
+        for (int i = lane; i < 32 * cols; i += 32) {
+            const int r = i / cols, c = i % cols, m = m0 + q * 32 + r, n = n0 + c0 + c;
+            if (m < p.rows && n < p.N) {
+                float y = stage[r * (cols + 1) + c];
+                if (p.residual) y += __bfloat162float(p.residual[m * p.res_stride + n]);
+                p.out[m * p.out_stride + n] = __float2bfloat16_rn(y);
+            }
+        }
+    }
+    // After a timeout copies may still be landing here: give them time (about
+    // 0.2 ms) before the shared memory is released.
+    if (threadIdx.x == 0 && aborted(bs)) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 400000) {
+        }
+    }
+    __syncwarp();
+    tc::cluster_sync();  // the others have read this CTA's sums
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, BN);
+    }
+}
+
+// ---------------------------------------------------------------------------- linear_pair
+namespace {
+constexpr int kPairM = 256, kPairN = 256;  // tile of a pair; each CTA holds 128 rows of both operands
+constexpr uint32_t kPairHalf = 128 * kSliceBytes;  // 16 KB
+constexpr uint32_t kPairStage = 2 * kPairHalf;
+constexpr int kPairStages = 6;
+constexpr int kEpiCols = 64;                        // output columns per epilogue step: one box of 32 rows
+constexpr uint32_t kBoxBytes = 32 * 128;
+constexpr uint32_t kOffBox = kPairStages * kPairStage;   // 2 boxes per epilogue warp
+constexpr uint32_t kOffPairBars = kOffBox + 8 * kBoxBytes;
+constexpr uint32_t kPairSmem = kOffPairBars + 512 + 1024;
+constexpr uint32_t kPairTmem = 2 * kPairN;
+static_assert(kPairSmem <= 232448, "shared memory budget");
+
+struct PairBars : BarsCommon {
+    uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], res[4][2], drain;
+};
+static_assert(sizeof(PairBars) <= 512, "barrier block");
+}  // namespace
+
+template <bool E4M3, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_pair(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
+                const __grid_constant__ CUtensorMap tg, const __grid_constant__ CUtensorMap tres,
+                const __grid_constant__ CUtensorMap tout, const LinParams p) {
+    constexpr int kOut = GATED ? kPairN / 2 : kPairN;
+    constexpr int kSteps = kOut / kEpiCols;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    PairBars *bs = reinterpret_cast<PairBars *>(sm + kOffPairBars);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_rank();
+    const int unit = (int)tc::cluster_id(), units = (int)tc::cluster_count();
+    const int total = p.m_tiles * p.n_tiles;
+    const int my_tiles = unit < total ? (total - 1 - unit) / units + 1 : 0;
+    clear_status(p.status);
+    if (my_tiles == 0) return;  // both CTAs of the pair
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) {
+            tc::mbar_init(&bs->full[s], 1);
+            tc::mbar_init(&bs->empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(&bs->acc_full[b], 1);
+            tc::mbar_init(&bs->acc_empty[b], 8);  // one arrival per epilogue warp of both CTAs
+            for (int w = 0; w < 4; ++w) tc::mbar_init(&bs->res[w][b], 1);
+        }
+        tc::mbar_init(&bs->drain, 1);
+        bs->abort = 0;
+        tc::fence_barrier_init();
+    }
+    if (warp == 1) {
+        tc::tmem_alloc_pair(&bs->tmem_base, kPairTmem);
+        tc::tmem_relinquish_pair();
+    }
+    tc::tc_fence_before();
+    tc::cluster_sync();  // the even CTA's barriers are ready before the peer signals them
+    tc::tc_fence_after();
+    const uint32_t tmem = bs->tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
+            // B rows of this CTA: gated, the even CTA stages the gate's rows and the odd one the weight's
+            const CUtensorMap *tb = GATED && rank == 0 ? &tg : &tw;
+            int it = 0;
+            bool ok = true;
+            for (int i = 0; i < my_tiles && ok; ++i) {
+                const int t = unit + i * units;
+                const int m0 = (t % p.m_tiles) * kPairM + (int)rank * 128;
+                const int nb = (t / p.m_tiles) * kOut + (GATED ? 0 : (int)rank * 128);
+                for (int kb = 0; kb < p.slices; ++kb) {
+                    const int s = it % kPairStages, use = it / kPairStages;
+                    if (use > 0 && !(ok = wait_or_abort(&bs->empty[s], (use - 1) & 1, bs, p.status))) break;
+                    if (aborted(bs)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *a = sm + s * kPairStage;
+                    const uint32_t fb = tc::cluster_addr(&bs->full[s], 0);
+                    if (rank == 0) tc::mbar_arrive_expect_tx(&bs->full[s], 2 * kPairStage);
+                    tc::tma_load_2d_pair(a, &tx, fb, kb * kElems, m0);
+                    tc::tma_load_2d_pair(a + kPairHalf, tb, fb, kb * kElems, nb);
+                    ++it;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = E4M3 ? tc::idesc_e4m3_f32(kPairM, kPairN) : tc::idesc_bf16_f32(kPairM, kPairN, false);
+            int it = 0;
+            bool ok = true;
+            for (int i = 0; i < my_tiles && ok; ++i) {
+                const int buf = i & 1, use = i >> 1;
+                if (use > 0 && !(ok = wait_or_abort(&bs->acc_empty[buf], (use - 1) & 1, bs, p.status))) break;
+                tc::tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(buf * kPairN);
+                for (int kb = 0; kb < p.slices; ++kb) {
+                    const int s = it % kPairStages;
+                    if (!(ok = wait_or_abort(&bs->full[s], (it / kPairStages) & 1, bs, p.status))) break;
+                    tc::tc_fence_after();
+                    const uint32_t a = tc::smem_u32(sm + s * kPairStage), b = a + kPairHalf;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t ad = tc::sdesc_sw128(a + kk * 32, 16, 1024), bd = tc::sdesc_sw128(b + kk * 32, 16, 1024);
+                        if constexpr (E4M3) tc::mma_e4m3_ss_pair(d, ad, bd, idesc, (kb | kk) != 0);
+                        else tc::mma_bf16_ss_pair(d, ad, bd, idesc, (kb | kk) != 0);
+                    }
+                    tc::mma_commit_pair_both(&bs->empty[s]);
+                    ++it;
+                }
+                if (ok) tc::mma_commit_pair_both(&bs->acc_full[buf]);
+            }
+            tc::mma_commit_pair(&bs->drain);
+            tc::mbar_wait(&bs->drain, 0, kWaitBudget);
+        }
+        __syncwarp();
+    } else {
+        // epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31; a step is 64 output
+        // columns of its 32 rows, one box (128 bytes a row, 128-byte swizzle) that
+        // the residual comes in by and the outputs leave by; two boxes in turn
+        const int q = warp & 3;
+        const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+        uint8_t *box = sm + kOffBox + q * 2 * kBoxBytes;
+        int step = 0;  // steps done: box step & 1, use step >> 1
+        auto load_residual = [&](int b, int n, int m) {  // lane 0
+            tc::mbar_arrive_expect_tx(&bs->res[q][b], kBoxBytes);
+            tc::tma_load_2d(box + b * kBoxBytes, &tres, &bs->res[q][b], n, m);
+        };
+        bool ok = true;
+        for (int i = 0; i < my_tiles && ok; ++i) {
+            const int t = unit + i * units;
+            const int mw = (t % p.m_tiles) * kPairM + (int)rank * 128 + q * 32, n0 = (t / p.m_tiles) * kOut;
+            const int buf = i & 1, m = mw + lane;
+            if (p.tma_res && lane == 0) {  // the residual's first box under the wait for the accumulator
+                tc::bulk_wait_read_all();
+                load_residual(step & 1, n0, mw);
+            }
+            ok = __all_sync(0xffffffffu, wait_or_abort(&bs->acc_full[buf], (i >> 1) & 1, bs, p.status));
+            if (!ok) {  // the residual's copy must land before this CTA may leave
+                if (p.tma_res && lane == 0) tc::mbar_wait(&bs->res[q][step & 1], (step >> 1) & 1, kWaitBudget);
+                break;
+            }
+            tc::tc_fence_after();
+            const float xs = E4M3 && m < p.rows ? __ldg(p.x_scale + m) : 1.0f;
+#pragma unroll 1
+            for (int h = 0; h < kSteps; ++h, ++step) {
+                const int b = step & 1, n = n0 + h * kEpiCols;
+                float v[64], u[GATED ? 64 : 1];
+                if constexpr (GATED) {  // columns 0 .. 127: gate, 128 .. 255: weight
+                    tc::tmem_ld64(tmem + lane_base + (uint32_t)(buf * kPairN + h * kEpiCols), u);
+                    tc::tmem_ld64(tmem + lane_base + (uint32_t)(buf * kPairN + kOut + h * kEpiCols), v);
+                } else {
+                    tc::tmem_ld64(tmem + lane_base + (uint32_t)(buf * kPairN + h * kEpiCols), v);
+                }
+                if (h == kSteps - 1) {  // the accumulator is in registers: the next tile may use it
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive_cluster(tc::cluster_addr(&bs->acc_empty[buf], 0));
+                }
+#pragma unroll
+                for (int e = 0; e < 64; ++e) {
+                    const Column c = column<GATED>(p.col, min(n + e, p.N - 1));  // same column in every lane
+                    v[e] = finish<GATED>(v[e], GATED ? u[e] : 0.0f, xs, c, p.act);
+                }
+                uint8_t *bx = box + b * kBoxBytes;
+                if (p.tma_out) {
+                    const uint32_t srow = tc::smem_u32(bx) + (uint32_t)lane * 128u;
+                    if (p.tma_res) {
+                        if (h + 1 < kSteps && lane == 0) {  // the next box: its last store has been read
+                            tc::bulk_wait_read_all();
+                            load_residual(b ^ 1, n + kEpiCols, mw);
+                        }
+                        __syncwarp();
+                        if (!(ok = __all_sync(0xffffffffu, wait_or_abort(&bs->res[q][b], (step >> 1) & 1, bs, p.status)))) break;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const uint4 r = *reinterpret_cast<const uint4 *>(bx + lane * 128 + ((c ^ (lane & 7)) << 4));
+                            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                v[8 * c + 2 * e] += bf16lo(w[e]);
+                                v[8 * c + 2 * e + 1] += bf16hi(w[e]);
+                            }
+                        }
+                    } else {
+                        if (lane == 0) tc::bulk_wait_read_but1();  // the store of two steps ago
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = tc::cvt_bf16x2(v[8 * c + 2 * e], v[8 * c + 2 * e + 1]);
+                        tc::st_shared_v4(srow + (((uint32_t)c ^ (uint32_t)(lane & 7)) << 4), w);
+                    }
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {  // clipped at the last column and row
+                        tc::tma_store_2d(&tout, bx, n, mw);
+                        tc::bulk_commit_group();
+                    }
+                } else {
+                    // rows that no tensor map can describe (odd pitch or width): through
+                    // shared memory (both boxes, fp32, 32 columns at a time), then 32
+                    // consecutive columns of a row per access
+                    float *st = reinterpret_cast<float *>(box);
+#pragma unroll
+                    for (int e0 = 0; e0 < 64; e0 += 32) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) st[lane * 33 + e] = v[e0 + e];
+                        __syncwarp();
+                        const int c = n + e0 + lane;
+                        if (c < p.N)
+                            for (int r = 0; r < 32 && mw + r < p.rows; ++r) {
+                                float y = st[r * 33 + lane];
+                                const int64_t mr = mw + r;
+                                if (p.residual) y += __bfloat162float(p.residual[mr * p.res_stride + c]);
+                                p.out[mr * p.out_stride + c] = __float2bfloat16_rn(y);
+                            }
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+        if (lane == 0) tc::bulk_wait_all();
+        __syncwarp();
+    }
+    if (threadIdx.x == 0 && aborted(bs)) {  // as in linear_tile
+        const long long t0 = clock64();
+        while (clock64() - t0 < 400000) {
+        }
+    }
+    __syncwarp();
+    tc::tc_fence_before();
+    tc::cluster_sync();  // the pair's MMAs and remote arrivals are over
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc_pair(tmem, kPairTmem);
+    }
+}
+
+// ---------------------------------------------------------------------------- host side
+namespace {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
+
+// 2-D row-major [outer][inner] of bf16 or bytes, pitch in elements, boxes of 128 bytes x box_rows, 128-byte swizzle.
+bool encode(CUtensorMap *map, bool bytes, const void *base, int64_t inner, int64_t outer, int64_t pitch, uint32_t box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const int es = bytes ? 1 : 2;
+    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+    // with one row the pitch is never used; it must still be a valid one
+    const cuuint64_t str[1] = {(cuuint64_t)pitch * es};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / es), box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base),
+              dims, str, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int device_sms() {
+    static std::atomic<int> n{0};
+    int v = n.load();
+    if (!v) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            v = 148;
+        n.store(v);
+    }
+    return v;
+}
+
+// What a tiling costs, in cycles: waves of tiles, each its K slices and what a
+// tile spends besides (filling the ring, the epilogue).
+struct Plan {
+    int bn = 0, split = 1;  // bn 0: linear_pair
+    double cost = 1e300;
+};
+Plan choose(const LinearArgs &a, int slices, int sms) {
+    Plan best;
+    const auto tiles = [&](int m, int n) {
+        return (long long)((a.rows + m - 1) / m) * ((a.N + n - 1) / n);
+    };
+    {
+        const long long t = tiles(kPairM, a.gate ? kPairN / 2 : kPairN);
+        const double waves = (double)((t + sms / 2 - 1) / (sms / 2));
+        best.cost = waves * (slices * 540.0) + 5000.0;
+    }
+    for (int bn : {64, 128})
+        for (int split : {1, 2, 4, 8}) {
+            if (split > 1 && split > slices) break;
+            const long long t = tiles(kTileM, a.gate ? bn / 2 : bn) * split;
+            const double waves = (double)((t + sms - 1) / sms);
+            const double per = (slices + split - 1) / split;
+            const double cost = waves * (per * (bn == 64 ? 400.0 : 540.0) + 3500.0 + (split > 1 ? 1500.0 : 0.0));
+            if (cost < best.cost) {
+                best.cost = cost;
+                best.bn = bn;
+                best.split = split;
+            }
+        }
+    return best;
+}
+
+template <bool E4M3, bool GATED, int BN>
+cudaError_t launch_tile(const LinearArgs &a, LinParams p, int split, cudaStream_t s) {
+    constexpr int kOut = GATED ? BN / 2 : BN;
+    CUtensorMap tx, tw, tg;
+    if (!encode(&tx, E4M3, a.x, a.K, a.rows, a.x_stride, kTileM)) return cudaErrorInvalidValue;
+    if (!encode(&tw, E4M3, a.weight, a.K, a.N, a.K, kOut)) return cudaErrorInvalidValue;
+    tg = tw;
+    if (GATED && !encode(&tg, E4M3, a.gate, a.K, a.N, a.K, kOut)) return cudaErrorInvalidValue;
+    p.m_tiles = (a.rows + kTileM - 1) / kTileM;
+    p.n_tiles = (a.N + kOut - 1) / kOut;
+    p.split = split;
+    auto kernel = linear_tile<E4M3, GATED, BN>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<BN>::kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((long long)p.m_tiles * p.n_tiles * split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = TileShape<BN>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, tg, p);
+}
+
+// CTA pairs that can be resident at once (one CTA per SM; an odd SM of a group stays out).
+template <typename K>
+int pair_slots(K kernel, const cudaLaunchConfig_t &cfg, int sms) {
+    static std::atomic<int> n{0};  // the same for every instantiation of the kernel: one CTA per SM by shared memory
+    int v = n.load();
+    if (!v) {
+        if (cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) != cudaSuccess || v < 1) v = sms / 2;
+        n.store(v);
+    }
+    return v;
+}
+
+template <bool E4M3, bool GATED>
+cudaError_t launch_pair(const LinearArgs &a, LinParams p, int sms, cudaStream_t s) {
+    constexpr int kOut = GATED ? kPairN / 2 : kPairN;
+    CUtensorMap tx, tw, tg, tres, tout;
+    if (!encode(&tx, E4M3, a.x, a.K, a.rows, a.x_stride, 128)) return cudaErrorInvalidValue;
+    if (!encode(&tw, E4M3, a.weight, a.K, a.N, a.K, 128)) return cudaErrorInvalidValue;
+    tg = tres = tout = tw;
+    if (GATED && !encode(&tg, E4M3, a.gate, a.K, a.N, a.K, 128)) return cudaErrorInvalidValue;
+    auto mappable = [&](const void *ptr, int64_t stride) {
+        return a.N % 8 == 0 && stride % 8 == 0 && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0;
+    };
+    p.tma_out = mappable(a.out, a.out_stride) && (!a.residual || mappable(a.residual, a.res_stride));
+    p.tma_res = p.tma_out && a.residual;
+    if (p.tma_out && !encode(&tout, false, a.out, a.N, a.rows, a.out_stride, 32)) return cudaErrorInvalidValue;
+    if (p.tma_res && !encode(&tres, false, a.residual, a.N, a.rows, a.res_stride, 32)) return cudaErrorInvalidValue;
+    p.m_tiles = (a.rows + kPairM - 1) / kPairM;
+    p.n_tiles = (a.N + kOut - 1) / kOut;
+    auto kernel = linear_pair<E4M3, GATED>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(2 * (sms / 2)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)(2 * std::min<long long>((long long)p.m_tiles * p.n_tiles, pair_slots(kernel, cfg, sms))));
+    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, tg, tres, tout, p);
+}
+
+template <bool E4M3, bool GATED>
+cudaError_t launch_type(const LinearArgs &a, cudaStream_t s) {
+    LinParams p{};
+    p.x_scale = a.x_scale;
+    p.col = {a.w_scale, a.g_scale, static_cast<const __nv_bfloat16 *>(a.bias), static_cast<const __nv_bfloat16 *>(a.g_bias)};
+    p.residual = static_cast<const __nv_bfloat16 *>(a.residual);
+    p.out = static_cast<__nv_bfloat16 *>(a.out);
+    p.res_stride = a.res_stride;
+    p.out_stride = a.out_stride;
+    p.rows = a.rows;
+    p.N = a.N;
+    p.act = a.act;
+    p.status = a.status;
+    const int elems = E4M3 ? kSliceBytes : kSliceBytes / 2;
+    p.slices = (a.K + elems - 1) / elems;
+    const int sms = device_sms();
+    const Plan plan = choose(a, p.slices, sms);
+    if (plan.bn == 0) return launch_pair<E4M3, GATED>(a, p, sms, s);
+    return plan.bn == 64 ? launch_tile<E4M3, GATED, 64>(a, p, plan.split, s)
+                         : launch_tile<E4M3, GATED, 128>(a, p, plan.split, s);
+}
+}  // namespace
+
+cudaError_t launch_linear(const LinearArgs &a, cudaStream_t s) {
+    if (a.rows <= kSkinnyRows) return launch_linear_skinny(a, s);
+    if (a.e4m3) return a.gate ? launch_type<true, true>(a, s) : launch_type<true, false>(a, s);
+    return a.gate ? launch_type<false, true>(a, s) : launch_type<false, false>(a, s);
+}
+
+}  // namespace a11s

@@ -1,7 +1,7 @@
 /*
  * a11spec.h - C ABI of the B200 speculative-decoding hot path.
  *
- * Five device steps, all asynchronous on the caller's
+ * Device steps, all asynchronous on the caller's
  * CUDA stream (passed as `void *stream`, a cudaStream_t; NULL = legacy
  * default stream):
  *
@@ -14,6 +14,9 @@
  *   a11s_ngram_update     the n-gram table learns committed tokens    (K6)
  *   a11s_next_roots       next roots and committed-token rows of a step (K6 input)
  *   a11s_lm_head          tree-node LM head, chunk records in its epilogue (K7)
+ *   a11s_add_rms_norm     residual addition + norm of a decoder layer     (K8)
+ *   a11s_linear           projections with their epilogue, bf16 or e4m3   (K9)
+ *   a11s_chunk_attention  attention of new tokens over the paged cache   (K10)
  *
  * Conventions shared by every entry point
  *   - All tensor arguments are caller-owned DEVICE pointers, row-major and
@@ -67,6 +70,12 @@ extern "C" {
 /* Element types. */
 #define A11S_F32  0
 #define A11S_BF16 1
+#define A11S_E4M3 2   /* 8-bit floating point, 4 exponent and 3 mantissa bits, largest value 448 */
+
+/* Activations of a11s_linear. */
+#define A11S_ACT_NONE 0
+#define A11S_ACT_SILU 1  /* v / (1 + exp(-v)) */
+#define A11S_ACT_GELU 2  /* v (1 + erf(v / sqrt(2))) / 2 */
 
 /* Acceptance modes for a11s_accept. */
 #define A11S_ACCEPT_GREEDY       0  /* accept child iff its token == argmax(parent row) */
@@ -260,6 +269,92 @@ int a11s_tree_attention(const void *q, const void *k_pool, const void *v_pool, i
                         int32_t head_dim, int32_t max_kv_len, float scale,
                         void *out, float *lse,
                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* ----------------------------------------------------------------------- K10
+ * Attention of a chunk of new tokens over the paged KV pool: the decode
+ * attention of engine/pipeline.py:386-402 for a prompt chunk of any length, or
+ * for one token per sequence.
+ *
+ * q    bf16 [batch][max_new][num_q_heads][head_dim], tokens q_stride elements apart
+ *   (>= num_q_heads * head_dim, a multiple of 8: q may be part of a fused q, k, v
+ *   projection's rows)
+ * k_pool, v_pool, page_table as for a11s_tree_attention.
+ * ctx_lens[b] >= 0: tokens before the chunk. n_new[b] in [0, max_new] (NULL:
+ *   max_new everywhere): live tokens of the chunk; token i's own K/V sit at
+ *   logical position ctx_lens[b] + i, and it sees the positions
+ *   0 .. ctx_lens[b] + i.
+ * out  bf16, as q but dense; lse fp32 [batch][max_new][num_q_heads], natural-log sum-exp of
+ *   the scaled scores (nullable). Rows i >= n_new[b] are written as zeros.
+ * Implemented: head_dim 64 or 128, num_q_heads a multiple of num_kv_heads, at
+ * most 128 query heads per KV head. max_kv_len >= every ctx_lens[b] + n_new[b]
+ * sizes the split of long caches (a smaller value costs speed, not results);
+ * page_table holds at least that many positions.
+ * Pool positions past ctx_lens[b] + n_new[b] - 1 never reach a result, whatever
+ * they hold. A non-finite V row of a live token may reach the rows of earlier
+ * tokens of its 128-key block (0 x Inf in the product).
+ * Device errors (status word): A11S_EBOUNDS with detail b for a page id outside
+ * the pool (its keys count as zeros) and for lengths outside the ranges above or
+ * beyond the page table (the sequence's rows are zeros); A11S_ETIMEOUT.
+ * Calls that overlap on the GPU need workspaces of their own.
+ */
+size_t a11s_chunk_attention_workspace_bytes(int32_t batch, int32_t max_new, int32_t num_q_heads,
+                                            int32_t num_kv_heads, int32_t head_dim, int32_t max_kv_len);
+
+int a11s_chunk_attention(const void *q, int64_t q_stride, const void *k_pool, const void *v_pool, int32_t num_pages,
+                         const int32_t *page_table, int32_t max_pages_per_seq, const int32_t *ctx_lens,
+                         const int32_t *n_new, int32_t batch, int32_t max_new, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t max_kv_len, float scale, void *out,
+                         float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------ K8
+ * Residual addition and root-mean-square norm in one pass: `h = h + ...` and
+ * `_rms_norm(h)` of engine/pipeline.py:403-407, 322-324.
+ *
+ * Per row, in fp32: h = x + residual (residual nullable: h = x);
+ *   y = (h * weight) * rsqrt(sum(h^2) / dim + eps).
+ * x, residual and sum have the type `dtype` (A11S_F32 or A11S_BF16), and so has
+ * weight [dim]; rows are *_stride elements apart (>= dim).
+ * sum (nullable): h rounded to `dtype`; it may be x or residual (in place). The
+ *   norm is taken of the unrounded h.
+ * out of the type out_dtype: `dtype`, or A11S_E4M3 with scales[row] =
+ *   max(max|y| / 448, 2^-100) and out = y / scale, rounded to nearest even; then
+ *   scales fp32 [rows] is required. out may not overlap an input or sum.
+ * A row that holds a NaN or an infinity, or whose squares overflow fp32, gives
+ * what these formulas give. 1 <= dim <= A11S_NORM_MAX_DIM. Rows and strides that
+ * are multiples of 16 bytes, on 16-byte aligned tensors, run vectorised.
+ */
+#define A11S_NORM_MAX_DIM 16384
+int a11s_add_rms_norm(int32_t dtype, const void *x, int64_t x_stride, const void *residual,
+                      int64_t residual_stride, const void *weight, int32_t rows, int32_t dim, float eps,
+                      void *sum, int64_t sum_stride, int32_t out_dtype, void *out, int64_t out_stride,
+                      float *scales, void *stream);
+
+/* ------------------------------------------------------------------------ K9
+ * Matrix product with its epilogue: the projections of engine/pipeline.py:364-373,
+ * 403-405 and 407-447.
+ *
+ *   v = x weight^T (x_scale[row] weight_scale[col]) + bias[col]
+ *   u = x gate^T (x_scale[row] gate_scale[col]) + gate_bias[col]      (gate given)
+ *   out[row][col] = (gate ? act(u) * v : act(v)) + residual[row][col]
+ * in fp32, rounded to bf16 once (nearest even).
+ * dtype A11S_BF16: x bf16 [rows][in_dim], rows x_stride elements apart, weight
+ *   and gate bf16 [out_dim][in_dim] dense; no scales (NULL).
+ * dtype A11S_E4M3: the same in e4m3; x_scale fp32 [rows], weight_scale (and
+ *   gate_scale) fp32 [out_dim] are required.
+ * bias, gate_bias bf16 [out_dim] (nullable); residual bf16, rows residual_stride
+ * apart (nullable); out bf16, rows out_stride apart, may be residual itself but
+ * overlap no other input. activation: A11S_ACT_*.
+ * in_dim and x_stride multiples of 16 bytes, x, weight and gate 16-byte aligned;
+ * rows, out_dim, out_stride and residual_stride are free. The order of the sum
+ * over in_dim is fixed by the sizes: equal calls give equal bits.
+ * workspace (nullable, >= 256 bytes): the status word, A11S_ETIMEOUT if a
+ * pipeline wait of the kernel ran out; without it that is not reported.
+ */
+int a11s_linear(int32_t dtype, const void *x, int64_t x_stride, const float *x_scale, const void *weight,
+                const float *weight_scale, const void *gate, const float *gate_scale, const void *bias,
+                const void *gate_bias, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t activation,
+                const void *residual, int64_t residual_stride, void *out, int64_t out_stride,
+                void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ K4
  * In-place compaction of the accepted path. Replaces the host block-table
