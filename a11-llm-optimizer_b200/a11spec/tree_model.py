@@ -24,6 +24,18 @@ the page table (where a11s_kv_compact expects them); its attention sees the
 context and its own ancestors. A one-node tree is the reference's single-token
 decode step; the prompt is prefilled as chain trees of up to 64 tokens.
 
+With fused=True the layer runs on this library's operators instead of torch's:
+one projection for q, k and v, the gate and up projections with silu(gate) * up
+in one product, the down projection adding to the residual stream (all
+a11s_linear), and the norms (a11s_add_rms_norm; the one before the FFN adds the
+attention's output to h). The statements are the same, with fp32 from a
+product's sum or a norm's input to its one rounding. fused="e4m3" also holds the
+weights behind the norms (q, k, v, gate, up) in e4m3 with a scale per output
+row, and the norms hand over e4m3 rows with a scale each.
+
+Prompts longer than a tree run in chunks of any length through
+a11s_chunk_attention (prefill(chunk=...)).
+
 Weights use the reference's GGUF tensor names (token_embd.weight,
 blk.{i}.attn_q.weight, ..., output.weight), as its WeightStore serves them.
 """
@@ -88,6 +100,12 @@ def tree_depths(parents: torch.Tensor, n_nodes: torch.Tensor) -> torch.Tensor:
     return torch.where(live, depth, torch.zeros_like(depth))
 
 
+def e4m3_rows(w: torch.Tensor):
+    """(e4m3 values, fp32 scale per row) of a weight [N, K]: scale = max|row| / 448."""
+    scale = (w.float().abs().amax(dim=1) / 448.0).clamp_min(2.0 ** -100)
+    return (w.float() / scale[:, None]).to(torch.float8_e4m3fn), scale
+
+
 class TreeDecoder:
     """Decoder stack over token trees (see the module docstring).
 
@@ -97,9 +115,17 @@ class TreeDecoder:
     slabs) and a11s_tree_attention reads one layer of."""
 
     def __init__(self, tensors: Dict[str, torch.Tensor], cfg: DecoderConfig, num_pages: int, device="cuda",
-                 compute_dtype: torch.dtype = torch.bfloat16):
+                 compute_dtype: torch.dtype = torch.bfloat16, fused=False):
         if cfg.n_head % cfg.n_head_kv:
             raise ValueError("n_head must be a multiple of n_head_kv")
+        if fused not in (False, True, "e4m3"):
+            raise ValueError("fused must be False, True or 'e4m3'")
+        if fused:
+            per16 = 16 if fused == "e4m3" else 8
+            if compute_dtype != torch.bfloat16:
+                raise ValueError("fused layers compute in bfloat16")
+            if cfg.n_embd % per16 or cfg.n_ff % 8 or (cfg.n_head * cfg.head_dim) % 8:
+                raise ValueError(f"fused layers need n_embd a multiple of {per16}, n_ff and n_head * head_dim of 8")
         self.cfg = cfg
         self.device = torch.device(device)
         self.dtype = compute_dtype
@@ -111,6 +137,35 @@ class TreeDecoder:
         self.v_pool = torch.zeros_like(self.k_pool)
         self.forwards = 0
         self.last_chunk_keys = None  # chunk keys of the last forward's logits (K7), or None
+        self.fused = fused
+        self.layers = [self._fuse(f"blk.{l}.") for l in range(cfg.n_layers)] if fused else None
+
+    def _fuse(self, blk: str) -> dict:
+        """Keyword arguments of a layer's three a11s_linear calls behind the norms and of its o and down products."""
+        def take(name):
+            return self.w.pop(blk + name + ".weight"), self.w.pop(blk + name + ".bias", None)
+
+        (wq, bq), (wk, bk), (wv, bv) = take("attn_q"), take("attn_k"), take("attn_v")
+        bias = None
+        if any(b is not None for b in (bq, bk, bv)):
+            bias = torch.cat([b if b is not None else w.new_zeros(w.shape[0]) for w, b in ((wq, bq), (wk, bk), (wv, bv))])
+        gate, gate_bias = take("ffn_gate")
+        up, up_bias = take("ffn_up")
+        wo, bo = take("attn_output")
+        down, down_bias = take("ffn_down")
+        qkv = dict(weight=torch.cat([wq, wk, wv]), bias=bias)
+        ffn = dict(weight=up, bias=up_bias, gate=gate, gate_bias=gate_bias, activation="silu")
+        if self.fused == "e4m3":
+            qkv["weight"], qkv["weight_scale"] = e4m3_rows(qkv["weight"])
+            ffn["weight"], ffn["weight_scale"] = e4m3_rows(ffn["weight"])
+            ffn["gate"], ffn["gate_scale"] = e4m3_rows(ffn["gate"])
+        return dict(qkv=qkv, ffn=ffn, out=dict(weight=wo, bias=bo), down=dict(weight=down, bias=down_bias))
+
+    def _norm(self, x: torch.Tensor, name: str, residual=None, feeds_product: bool = True):
+        """(norm of x (+ residual) for a product, its scales, the sum)."""
+        e4m3 = self.fused == "e4m3" and feeds_product
+        return ops.add_rms_norm(x, self.w[name], residual=residual, eps=self.cfg.rms_eps,
+                                out_dtype=torch.float8_e4m3fn if e4m3 else None)
 
     def _proj(self, x: torch.Tensor, name: str) -> torch.Tensor:
         y = torch.matmul(x, self.w[name + ".weight"].t())
@@ -126,13 +181,31 @@ class TreeDecoder:
         self.k_pool[layer, page, off] = k[b, i].to(torch.bfloat16)
         self.v_pool[layer, page, off] = v[b, i].to(torch.bfloat16)
 
-    def _forward(self, tokens, parents, n_nodes, page_table, ctx_lens, positions):
-        cfg = self.cfg
+    def _forward(self, tokens, parents, n_nodes, page_table, ctx_lens, positions, max_kv_len=None):
+        """Logits of every token. With max_kv_len the tokens are a chunk (each
+        follows the one before it), else a tree of `parents`."""
         B, N = tokens.shape
         ar = torch.arange(N, device=tokens.device)
         live = ar.unsqueeze(0) < n_nodes.unsqueeze(1)
         slots = ctx_lens.long().unsqueeze(1) + ar.unsqueeze(0)
+
+        def attend(l, q, k, v):
+            q, k = rotary(q, k, positions, self.cfg.rope_base)
+            self._write_kv(l, k, v, slots, page_table, live)
+            q = q.to(torch.bfloat16).contiguous()
+            if max_kv_len is not None:
+                return ops.chunk_attention(q, self.k_pool[l], self.v_pool[l], page_table, ctx_lens, n_nodes,
+                                           max_kv_len=max_kv_len)[0]
+            return ops.tree_attention(q, self.k_pool[l], self.v_pool[l], page_table, ctx_lens, parents, n_nodes)[0]
+
         h = self.w["token_embd.weight"][tokens.clamp_min(0).long()]  # [B, N, n_embd]
+        hn = self._layers_fused(h, attend) if self.fused else self._layers(h, attend)
+        self.forwards += 1
+        return self._head(hn)
+
+    def _layers(self, h, attend):
+        cfg = self.cfg
+        B, N = h.shape[:2]
         for l in range(cfg.n_layers):
             blk = f"blk.{l}."
             hn = rms_norm(h, self.w[blk + "attn_norm.weight"], cfg.rms_eps)
@@ -143,17 +216,34 @@ class TreeDecoder:
                 q = rms_norm(q, self.w[blk + "attn_q_norm.weight"], cfg.rms_eps)
             if blk + "attn_k_norm.weight" in self.w:
                 k = rms_norm(k, self.w[blk + "attn_k_norm.weight"], cfg.rms_eps)
-            q, k = rotary(q, k, positions, cfg.rope_base)
-            self._write_kv(l, k, v, slots, page_table, live)
-            attn, _, _ = ops.tree_attention(q.to(torch.bfloat16).contiguous(), self.k_pool[l], self.v_pool[l],
-                                            page_table, ctx_lens, parents, n_nodes)
+            attn = attend(l, q, k, v)
             h = h + self._proj(attn.to(self.dtype).reshape(B, N, cfg.n_head * cfg.head_dim), blk + "attn_output")
             hf = rms_norm(h, self.w[blk + "ffn_norm.weight"], cfg.rms_eps)
             act = F.silu(self._proj(hf, blk + "ffn_gate")) * self._proj(hf, blk + "ffn_up")
             h = h + self._proj(act, blk + "ffn_down")
-        hn = rms_norm(h, self.w["output_norm.weight"], cfg.rms_eps)
-        self.forwards += 1
-        return self._head(hn)
+        return rms_norm(h, self.w["output_norm.weight"], cfg.rms_eps)
+
+    def _layers_fused(self, h, attend):
+        cfg = self.cfg
+        B, N = h.shape[:2]
+        dq, dk = cfg.n_head * cfg.head_dim, cfg.n_head_kv * cfg.head_dim
+        for l, w in enumerate(self.layers):
+            blk = f"blk.{l}."
+            hn, scales, _ = self._norm(h, blk + "attn_norm.weight")
+            qkv = ops.linear(hn, x_scale=scales, **w["qkv"])
+            q = qkv[..., :dq].view(B, N, cfg.n_head, cfg.head_dim)
+            k = qkv[..., dq:dq + dk].view(B, N, cfg.n_head_kv, cfg.head_dim)
+            v = qkv[..., dq + dk:].view(B, N, cfg.n_head_kv, cfg.head_dim)
+            if blk + "attn_q_norm.weight" in self.w:
+                q, _, _ = self._norm(q.contiguous(), blk + "attn_q_norm.weight", feeds_product=False)
+            if blk + "attn_k_norm.weight" in self.w:
+                k, _, _ = self._norm(k.contiguous(), blk + "attn_k_norm.weight", feeds_product=False)
+            attn = attend(l, q, k, v)
+            o = ops.linear(attn.view(B, N, dq), **w["out"])
+            hf, scales, h = self._norm(o, blk + "ffn_norm.weight", residual=h)
+            act = ops.linear(hf, x_scale=scales, **w["ffn"])
+            h = ops.linear(act, residual=h, **w["down"])
+        return self._norm(h, "output_norm.weight", feeds_product=False)[0]
 
     def _head(self, hn: torch.Tensor) -> torch.Tensor:
         """logits = hn output_w^T (engine/pipeline.py:469-472). A bf16 model
@@ -176,9 +266,10 @@ class TreeDecoder:
         return self._forward(tokens, parents, n_nodes, page_table, ctx_lens, pos).contiguous()
 
     def prefill(self, tokens, page_table, ctx_lens=None, chunk: int = 64) -> Optional[torch.Tensor]:
-        """K/V of the prompt tokens [B, T] at positions 0 .. T-1, as chain trees
-        of up to `chunk` tokens (each attends to the earlier chunks and to its
-        own prefix). Returns the logits of the last chunk."""
+        """K/V of the prompt tokens [B, T] at positions 0 .. T-1, in chunks of up
+        to `chunk` tokens (each attends to the earlier chunks and to its own
+        prefix): chain trees up to 64, a11s_chunk_attention beyond. Returns the
+        logits of the last chunk."""
         B, T = tokens.shape
         logits = None
         for c0 in range(0, T, chunk):
@@ -187,7 +278,8 @@ class TreeDecoder:
             nn = torch.full((B,), n, dtype=torch.int32, device=tokens.device)
             ctx = torch.full((B,), c0, dtype=torch.int32, device=tokens.device)
             pos = c0 + torch.arange(n, device=tokens.device).unsqueeze(0).expand(B, n)
-            logits = self._forward(tokens[:, c0:c0 + n].contiguous(), par, nn, page_table, ctx, pos)
+            logits = self._forward(tokens[:, c0:c0 + n].contiguous(), par, nn, page_table, ctx, pos,
+                                   max_kv_len=c0 + n if chunk > 64 else None)
         return logits
 
 
