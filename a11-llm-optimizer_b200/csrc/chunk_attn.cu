@@ -491,13 +491,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Merge of the splits of each live row, in split order: one warp per (b, token, head).
+// Merge of the splits of each live row, in split order: one block of D threads
+// per (b, token, head); the splits' weights first, one per thread.
 template <int D>
-__global__ void chunk_attn_combine(const Params p) {
-    const size_t row = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5, rows = (size_t)p.B * p.N * p.Hq;
-    const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
-    const int b = (int)(row / ((size_t)p.N * p.Hq)), token = (int)((row / p.Hq) % p.N);
+__global__ void __launch_bounds__(D) chunk_attn_combine(const Params p) {
+    __shared__ float weight[kMaxSplits];
+    __shared__ float total[2];
+    const size_t row = blockIdx.x, rows = (size_t)p.B * p.N * p.Hq;
+    const int t = threadIdx.x, b = (int)(row / ((size_t)p.N * p.Hq)), token = (int)((row / p.Hq) % p.N);
     int L;
     const int n_live = live_tokens(p, b, L, false);
     if (token >= n_live) return;  // its zeros are written
@@ -505,41 +506,41 @@ __global__ void chunk_attn_combine(const Params p) {
     const int per_cta = kTiles * p.tokens, last = min(n_live, (token / per_cta + 1) * per_cta) - 1;
     const int nblk = (L + last + kBlockKV) / kBlockKV;
     const int splits = min(p.splits, (nblk + p.split_blocks - 1) / p.split_blocks);
-    float acc[D / 32] = {};
-    float M = -INFINITY, wsum = 0.0f;
-    for (int s0 = 0; s0 < splits; s0 += 4) {
-        float ms[4], ls[4], o[4][D / 32];
+    const float *po = p.part_o + row * D + t;
+    if (t < 32) {  // weights 2^(m - M) l and their sum (each split's output is already divided by its l)
+        float m[kMaxSplits / 32], l[kMaxSplits / 32], M = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const size_t prow = (size_t)min(s0 + g, splits - 1) * rows + row;
-            ms[g] = p.part_ml[prow * 2];
-            ls[g] = s0 + g < splits ? p.part_ml[prow * 2 + 1] : 0.0f;
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e) o[g][e] = p.part_o[prow * D + e * 32 + lane];
+        for (int i = 0; i < kMaxSplits / 32; ++i) {
+            const int s = t + 32 * i;
+            const size_t at = ((size_t)min(s, splits - 1) * rows + row) * 2;
+            m[i] = p.part_ml[at];
+            l[i] = s < splits ? p.part_ml[at + 1] : 0.0f;
+            if (l[i] != 0.0f) M = fmaxf(M, m[i]);
         }
-        float Mg = M;
+        M = warp_fmax(M);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-            if (ls[g] != 0.0f) Mg = fmaxf(Mg, ms[g]);
-        if (Mg == -INFINITY) continue;
-        const float a = M == -INFINITY ? 0.0f : exp2f(M - Mg);
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] *= a;
-        wsum *= a;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            if (ls[g] == 0.0f) continue;
-            const float w = ls[g] * exp2f(ms[g] - Mg);
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(w, o[g][e], acc[e]);
-            wsum += w;
+        for (int i = 0; i < kMaxSplits / 32; ++i) {
+            const float w = l[i] == 0.0f ? 0.0f : l[i] * exp2f(m[i] - M);
+            weight[t + 32 * i] = w;
+            sum += w;
         }
-        M = Mg;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (t == 0) {
+            total[0] = sum;
+            total[1] = M;
+        }
     }
-    const float inv = wsum == 0.0f ? 0.0f : 1.0f / wsum;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) p.out[row * D + e * 32 + lane] = __float2bfloat16_rn(acc[e] * inv);
-    if (p.lse && lane == 0) p.lse[row] = wsum == 0.0f ? 0.0f : (M + log2f(wsum)) * 0.6931471805599453f;
+    __syncthreads();
+    float acc = 0.0f;
+#pragma unroll 16
+    for (int s = 0; s < splits; ++s) {
+        const float w = weight[s], o = po[(size_t)s * rows * D];
+        if (w != 0.0f) acc = fmaf(w, o, acc);
+    }
+    const float sum = total[0], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    p.out[row * D + t] = __float2bfloat16_rn(acc * inv);
+    if (p.lse && t == 0) p.lse[row] = sum == 0.0f ? 0.0f : (total[1] + log2f(sum)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -616,8 +617,7 @@ cudaError_t launch_d(const ChunkAttnArgs &a, const Params &p, cudaStream_t s) {
     kernel<<<(unsigned)((long long)p.ctiles * p.B * p.splits * p.Hkv), kThreads, Shape<D>::kSmem, s>>>(tk, tv, p);
     e = cudaGetLastError();
     if (e != cudaSuccess || p.splits == 1) return e;
-    const size_t rows = (size_t)p.B * p.N * p.Hq;
-    chunk_attn_combine<D><<<(unsigned)((rows * 32 + 127) / 128), 128, 0, s>>>(p);
+    chunk_attn_combine<D><<<(unsigned)((size_t)p.B * p.N * p.Hq), D, 0, s>>>(p);
     return cudaGetLastError();
 }
 }  // namespace

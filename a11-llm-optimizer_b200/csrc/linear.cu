@@ -50,7 +50,7 @@ struct LinParams {
     __nv_bfloat16 *out;
     int64_t res_stride, out_stride;
     int32_t rows, N, act, m_tiles, n_tiles, slices, split;
-    int32_t tma_out, tma_res;  // linear_pair: out (and the residual) take tensor maps
+    int32_t tma_out, vec_res;  // linear_pair: out takes a tensor map; residual rows are read 16 bytes at a time
     StatusWord *status;
 };
 
@@ -81,13 +81,39 @@ struct TileShape {
     static constexpr uint32_t kStage = kTileABytes + BN * kSliceBytes;
     static constexpr int kStages = BN == 64 ? 8 : 6;
     static constexpr uint32_t kRing = kStages * kStage;  // 192 KB
-    static constexpr uint32_t kSmem = kRing + 512 + 1024;
+    static constexpr uint32_t kOffCols = kRing;       // 4 x 128 column parameters
+    static constexpr uint32_t kOffBars = kRing + 2048;
+    static constexpr uint32_t kSmem = kOffBars + 512 + 1024;
 };
 struct TileBars : BarsCommon {
     uint64_t full[8], empty[8], acc_full, drain;
 };
 static_assert(sizeof(TileBars) <= 512, "barrier block");
 }  // namespace
+
+// Barrier of the epilogue warps only.
+template <int THREADS>
+__device__ __forceinline__ void epilogue_barrier() {
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
+// A warp's 32 rows of C consecutive outputs from shared memory (rows C + 1
+// floats apart): the residual is added and the row segments written coalesced.
+template <int C>
+__device__ __forceinline__ void write_rows(const float *stage, const LinParams &p, int m0, int n0, int lane) {
+    constexpr int kRows = C >= 32 ? 1 : 32 / C, kParts = C >= 32 ? C / 32 : 1;  // rows per access, accesses per row
+    const int r0 = C >= 32 ? 0 : lane / C, c0 = C >= 32 ? lane : lane % C;
+#pragma unroll 8
+    for (int i = 0; i < 32 / kRows * kParts; ++i) {
+        const int r = i / kParts * kRows + r0, c = c0 + (i % kParts) * 32;
+        const int64_t m = m0 + r;
+        const int n = n0 + c;
+        if (m < p.rows && n < p.N) {
+            float y = stage[r * (C + 1) + c];
+            if (p.residual) y += __bfloat162float(p.residual[m * p.res_stride + n]);
+            p.out[m * p.out_stride + n] = __float2bfloat16_rn(y);
+        }
+    }
+}
 
 // One 128 x BN tile (gated: 128 x BN/2 outputs) per cluster of p.split CTAs;
 // each CTA multiplies its share of the K slices.
@@ -99,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kOut = GATED ? BN / 2 : BN;  // output columns of a tile
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    TileBars *bs = reinterpret_cast<TileBars *>(sm + S::kRing);
+    TileBars *bs = reinterpret_cast<TileBars *>(sm + S::kOffBars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % p.split, tile = blockIdx.x / p.split;  // clusters are consecutive CTAs
     const int m0 = (tile % p.m_tiles) * kTileM, n0 = (tile / p.m_tiles) * kOut;
@@ -168,17 +194,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     }
-    // ---------------- the accumulator is complete: the ring is free ----------------
-    // part: this CTA's sums, [BN][128] fp32, column-major (a warp's 32 rows are
-    // consecutive); stage: finished outputs of an epilogue warp, [32][cols + 1] fp32
-    float *part = reinterpret_cast<float *>(sm);
-    const int q = warp & 3, row = q * 32 + lane;  // of epilogue warps: TMEM lane = tile row
+    // ---------------- epilogue warps ----------------
+    const int q = warp & 3, row = q * 32 + lane, m = m0 + row;  // TMEM lane = tile row
+    const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+    float *cols_sm = reinterpret_cast<float *>(sm + S::kOffCols);
+    const bool params = p.col.any();
+    float xs = 1.0f;
     bool ok = true;
     if (warp >= 2) {
+        if (params) stage_columns<GATED, kOut>(cols_sm, p.col, n0, p.N, threadIdx.x - 64, 128);
+        if (E4M3 && m < p.rows) xs = __ldg(p.x_scale + m);
+        epilogue_barrier<128>();
         ok = __all_sync(0xffffffffu, wait_or_abort(&bs->acc_full, 0, bs, p.status));
-        if (ok) {
-            tc::tc_fence_after();
-            const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+        tc::tc_fence_after();
+    }
+    // With the accumulator complete the ring is free. part: this CTA's sums,
+    // [BN][128] fp32, column-major; stage: finished outputs of an epilogue warp.
+    float *part = reinterpret_cast<float *>(sm);
+    float *stage = reinterpret_cast<float *>(sm + BN * kTileM * 4) + q * 32 * (kOut + 1);
+    if (p.split == 1) {
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (int c = 0; c < kOut; c += 32) {
+                float v[32], u[GATED ? 32 : 1];
+                tc::tmem_ld32(tmem + lane_base + (GATED ? kOut : 0) + c, v);
+                if constexpr (GATED) tc::tmem_ld32(tmem + lane_base + c, u);
+                finish_columns<GATED, kOut>(v, u, xs, cols_sm, c, params, p.act);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) stage[lane * 33 + e] = v[e];
+                __syncwarp();
+                write_rows<32>(stage, p, m0 + q * 32, n0 + c, lane);
+                __syncwarp();
+            }
+        }
+    } else {
+        if (warp >= 2 && ok) {
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
                 float v[32];
@@ -192,38 +242,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 32; ++e) part[(c + e) * kTileM + row] = v[e];
             }
         }
-    }
-    tc::tc_fence_before();
-    tc::cluster_sync();  // every CTA's sums are in shared memory (and after a timeout nobody waits for them)
-    if (warp >= 2 && ok) {
-        const int cols = kOut / p.split, c0 = rank * cols;  // this CTA's output columns of the tile
-        float *stage = reinterpret_cast<float *>(sm + BN * kTileM * 4) + q * 32 * (kOut + 1);
-        const float xs = E4M3 && m0 + row < p.rows ? __ldg(p.x_scale + m0 + row) : 1.0f;
-        uint32_t src[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) src[r] = r < p.split ? tc::cluster_addr(part, r) : 0;
-        for (int c = 0; c < cols; ++c) {
-            // gated: the gate's columns are the first half of the tile
-            const uint32_t at = ((GATED ? kOut : 0) + c0 + c) * kTileM + row, gat = (c0 + c) * kTileM + row;
-            float v = 0.0f, u = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (r < p.split) {
-                    v += tc::ld_cluster_f32(src[r] + at * 4);
-                    if (GATED) u += tc::ld_cluster_f32(src[r] + gat * 4);
-                }
-            const int n = n0 + c0 + c;
-            if (n < p.N) v = finish<GATED>(v, u, xs, column<GATED>(p.col, n), p.act);
-            stage[lane * (cols + 1) + c] = v;
-        }
         __syncwarp();
-        // rows of the warp, `cols` consecutive columns each, written coalesced
-        for (int i = lane; i < 32 * cols; i += 32) {
-            const int r = i / cols, c = i % cols, m = m0 + q * 32 + r, n = n0 + c0 + c;
-            if (m < p.rows && n < p.N) {
-                float y = stage[r * (cols + 1) + c];
-                if (p.residual) y += __bfloat162float(p.residual[m * p.res_stride + n]);
-                p.out[m * p.out_stride + n] = __float2bfloat16_rn(y);
+        tc::cluster_sync();  // every CTA's sums are in shared memory (and after a timeout nobody waits for them)
+        if (warp >= 2 && ok) {
+            const int cols = kOut / p.split, c0 = rank * cols;  // this CTA's output columns of the tile
+            uint32_t src[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) src[r] = tc::cluster_addr(part, r < p.split ? r : 0) + (uint32_t)row * 4;
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 4) {
+                // gated: the gate's columns are the first half of the tile
+                float v[4] = {}, u[4] = {};
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < p.split) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            v[e] += tc::ld_cluster_f32(src[r] + ((GATED ? kOut : 0) + c0 + c + e) * (kTileM * 4));
+                            if (GATED) u[e] += tc::ld_cluster_f32(src[r] + (c0 + c + e) * (kTileM * 4));
+                        }
+                    }
+                finish_columns<GATED, kOut>(v, u, xs, cols_sm, c0 + c, params, p.act);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) stage[lane * (cols + 1) + c + e] = v[e];
+            }
+            __syncwarp();
+            switch (cols) {
+                case 4: write_rows<4>(stage, p, m0 + q * 32, n0 + c0, lane); break;
+                case 8: write_rows<8>(stage, p, m0 + q * 32, n0 + c0, lane); break;
+                case 16: write_rows<16>(stage, p, m0 + q * 32, n0 + c0, lane); break;
+                case 32: write_rows<32>(stage, p, m0 + q * 32, n0 + c0, lane); break;
+                default: write_rows<64>(stage, p, m0 + q * 32, n0 + c0, lane); break;
             }
         }
     }
@@ -235,7 +284,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncwarp();
-    tc::cluster_sync();  // the others have read this CTA's sums
+    tc::tc_fence_before();
+    tc::cluster_sync();  // the others have read this CTA's sums; its TMEM loads are over
     if (warp == 1) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, BN);
@@ -245,28 +295,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------- linear_pair
 namespace {
 constexpr int kPairM = 256, kPairN = 256;  // tile of a pair; each CTA holds 128 rows of both operands
+constexpr int kPairThreads = 320;                  // TMA warp, MMA warp, 8 epilogue warps
+constexpr int kEpiThreads = kPairThreads - 64;
 constexpr uint32_t kPairHalf = 128 * kSliceBytes;  // 16 KB
 constexpr uint32_t kPairStage = 2 * kPairHalf;
 constexpr int kPairStages = 6;
-constexpr int kEpiCols = 64;                        // output columns per epilogue step: one box of 32 rows
-constexpr uint32_t kBoxBytes = 32 * 128;
-constexpr uint32_t kOffBox = kPairStages * kPairStage;   // 2 boxes per epilogue warp
-constexpr uint32_t kOffPairBars = kOffBox + 8 * kBoxBytes;
+constexpr int kEpiCols = 32;                       // output columns per epilogue step: a box of 32 rows x 64 bytes
+constexpr uint32_t kBoxPitch = 2560;               // 2 KB box (or 32 x 17 floats), on 512 bytes
+constexpr uint32_t kOffBox = kPairStages * kPairStage;       // one box per epilogue warp
+constexpr uint32_t kOffPairCols = kOffBox + 8 * kBoxPitch;   // column parameters of two tiles: 512 floats each
+constexpr uint32_t kOffPairBars = kOffPairCols + 4096;
 constexpr uint32_t kPairSmem = kOffPairBars + 512 + 1024;
 constexpr uint32_t kPairTmem = 2 * kPairN;
-static_assert(kPairSmem <= 232448, "shared memory budget");
+static_assert(kPairSmem <= 232448 && 32 * 17 * 4 <= kBoxPitch, "shared memory budget");
 
 struct PairBars : BarsCommon {
-    uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], res[4][2], drain;
+    uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], drain;
 };
 static_assert(sizeof(PairBars) <= 512, "barrier block");
 }  // namespace
 
 template <bool E4M3, bool GATED>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     linear_pair(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
-                const __grid_constant__ CUtensorMap tg, const __grid_constant__ CUtensorMap tres,
-                const __grid_constant__ CUtensorMap tout, const LinParams p) {
+                const __grid_constant__ CUtensorMap tg, const __grid_constant__ CUtensorMap tout, const LinParams p) {
     constexpr int kOut = GATED ? kPairN / 2 : kPairN;
     constexpr int kSteps = kOut / kEpiCols;
     extern __shared__ uint8_t smem_raw[];
@@ -287,8 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             tc::mbar_init(&bs->acc_full[b], 1);
-            tc::mbar_init(&bs->acc_empty[b], 8);  // one arrival per epilogue warp of both CTAs
-            for (int w = 0; w < 4; ++w) tc::mbar_init(&bs->res[w][b], 1);
+            tc::mbar_init(&bs->acc_empty[b], 16);  // one arrival per epilogue warp of both CTAs
         }
         tc::mbar_init(&bs->drain, 1);
         bs->abort = 0;
@@ -362,108 +413,87 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else {
-        // epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31; a step is 64 output
-        // columns of its 32 rows, one box (128 bytes a row, 128-byte swizzle) that
-        // the residual comes in by and the outputs leave by; two boxes in turn
-        const int q = warp & 3;
+        // epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 and takes every other
+        // step (w / 4) of 32 output columns. The outputs leave through a box of its
+        // own (64 bytes a row, 64-byte swizzle) by TMA stores.
+        const int q = warp & 3, first = (warp - 2) >> 2;
         const uint32_t lane_base = (uint32_t)(q * 32) << 16;
-        uint8_t *box = sm + kOffBox + q * 2 * kBoxBytes;
-        int step = 0;  // steps done: box step & 1, use step >> 1
-        auto load_residual = [&](int b, int n, int m) {  // lane 0
-            tc::mbar_arrive_expect_tx(&bs->res[q][b], kBoxBytes);
-            tc::tma_load_2d(box + b * kBoxBytes, &tres, &bs->res[q][b], n, m);
-        };
+        uint8_t *box = sm + kOffBox + (warp - 2) * kBoxPitch;
+        const uint32_t srow = tc::smem_u32(box) + (uint32_t)lane * 64u;
+        const bool params = p.col.any();
         bool ok = true;
         for (int i = 0; i < my_tiles && ok; ++i) {
             const int t = unit + i * units;
             const int mw = (t % p.m_tiles) * kPairM + (int)rank * 128 + q * 32, n0 = (t / p.m_tiles) * kOut;
             const int buf = i & 1, m = mw + lane;
-            if (p.tma_res && lane == 0) {  // the residual's first box under the wait for the accumulator
-                tc::bulk_wait_read_all();
-                load_residual(step & 1, n0, mw);
+            float *cols = reinterpret_cast<float *>(sm + kOffPairCols) + buf * 512;
+            float xs = 1.0f;
+            // under the wait for the accumulator: the tile's column parameters (the
+            // buffer's readers, two tiles back, passed the barrier of the tile between)
+            if (params) {
+                stage_columns<GATED, kOut>(cols, p.col, n0, p.N, threadIdx.x - 64, kEpiThreads);
+                epilogue_barrier<kEpiThreads>();
             }
+            if (E4M3 && m < p.rows) xs = __ldg(p.x_scale + m);
+            uint4 res[4];
+            auto load_residual = [&](int n) {  // this row's 32 columns at n; absent ones are never stored
+                const bool in = m < p.rows;
+                const uint4 *src = reinterpret_cast<const uint4 *>(p.residual + (int64_t)m * p.res_stride + n);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) res[c] = in && n + 8 * c < p.N ? __ldcs(src + c) : make_uint4(0, 0, 0, 0);
+            };
+            if (p.vec_res) load_residual(n0 + first * kEpiCols);
             ok = __all_sync(0xffffffffu, wait_or_abort(&bs->acc_full[buf], (i >> 1) & 1, bs, p.status));
-            if (!ok) {  // the residual's copy must land before this CTA may leave
-                if (p.tma_res && lane == 0) tc::mbar_wait(&bs->res[q][step & 1], (step >> 1) & 1, kWaitBudget);
-                break;
-            }
+            if (!ok) break;
             tc::tc_fence_after();
-            const float xs = E4M3 && m < p.rows ? __ldg(p.x_scale + m) : 1.0f;
 #pragma unroll 1
-            for (int h = 0; h < kSteps; ++h, ++step) {
-                const int b = step & 1, n = n0 + h * kEpiCols;
-                float v[64], u[GATED ? 64 : 1];
-                if constexpr (GATED) {  // columns 0 .. 127: gate, 128 .. 255: weight
-                    tc::tmem_ld64(tmem + lane_base + (uint32_t)(buf * kPairN + h * kEpiCols), u);
-                    tc::tmem_ld64(tmem + lane_base + (uint32_t)(buf * kPairN + kOut + h * kEpiCols), v);
-                } else {
-                    tc::tmem_ld64(tmem + lane_base + (uint32_t)(buf * kPairN + h * kEpiCols), v);
-                }
-                if (h == kSteps - 1) {  // the accumulator is in registers: the next tile may use it
+            for (int h = first; h < kSteps; h += 2) {
+                const int n = n0 + h * kEpiCols;
+                float v[32], u[GATED ? 32 : 1];
+                if constexpr (GATED) tc::tmem_ld32(tmem + lane_base + (uint32_t)(buf * kPairN + h * kEpiCols), u);
+                tc::tmem_ld32(tmem + lane_base + (uint32_t)(buf * kPairN + (GATED ? kOut : 0) + h * kEpiCols), v);
+                if (h + 2 >= kSteps) {  // the accumulator is in registers: the next tile may use it
                     tc::tc_fence_before();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive_cluster(tc::cluster_addr(&bs->acc_empty[buf], 0));
                 }
-#pragma unroll
-                for (int e = 0; e < 64; ++e) {
-                    const Column c = column<GATED>(p.col, min(n + e, p.N - 1));  // same column in every lane
-                    v[e] = finish<GATED>(v[e], GATED ? u[e] : 0.0f, xs, c, p.act);
-                }
-                uint8_t *bx = box + b * kBoxBytes;
+                finish_columns<GATED, kOut>(v, u, xs, cols, h * kEpiCols, params, p.act);
                 if (p.tma_out) {
-                    const uint32_t srow = tc::smem_u32(bx) + (uint32_t)lane * 128u;
-                    if (p.tma_res) {
-                        if (h + 1 < kSteps && lane == 0) {  // the next box: its last store has been read
-                            tc::bulk_wait_read_all();
-                            load_residual(b ^ 1, n + kEpiCols, mw);
-                        }
-                        __syncwarp();
-                        if (!(ok = __all_sync(0xffffffffu, wait_or_abort(&bs->res[q][b], (step >> 1) & 1, bs, p.status)))) break;
+                    if (p.vec_res) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const uint4 r = *reinterpret_cast<const uint4 *>(bx + lane * 128 + ((c ^ (lane & 7)) << 4));
-                            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t w[4] = {res[c].x, res[c].y, res[c].z, res[c].w};
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 v[8 * c + 2 * e] += bf16lo(w[e]);
                                 v[8 * c + 2 * e + 1] += bf16hi(w[e]);
                             }
                         }
-                    } else {
-                        if (lane == 0) tc::bulk_wait_read_but1();  // the store of two steps ago
-                        __syncwarp();
+                        if (h + 2 < kSteps) load_residual(n + 2 * kEpiCols);
                     }
+                    if (lane == 0) tc::bulk_wait_read_all();  // the box's last store
+                    __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
+                    for (int c = 0; c < 4; ++c) {
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) w[e] = tc::cvt_bf16x2(v[8 * c + 2 * e], v[8 * c + 2 * e + 1]);
-                        tc::st_shared_v4(srow + (((uint32_t)c ^ (uint32_t)(lane & 7)) << 4), w);
+                        tc::st_shared_v4(srow + (((uint32_t)c ^ (uint32_t)((lane >> 1) & 3)) << 4), w);
                     }
                     tc::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {  // clipped at the last column and row
-                        tc::tma_store_2d(&tout, bx, n, mw);
+                        tc::tma_store_2d(&tout, box, n, mw);
                         tc::bulk_commit_group();
                     }
-                } else {
-                    // rows that no tensor map can describe (odd pitch or width): through
-                    // shared memory (both boxes, fp32, 32 columns at a time), then 32
-                    // consecutive columns of a row per access
+                } else {  // rows that no tensor map can describe (odd pitch or width)
                     float *st = reinterpret_cast<float *>(box);
 #pragma unroll
-                    for (int e0 = 0; e0 < 64; e0 += 32) {
+                    for (int e0 = 0; e0 < 32; e0 += 16) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) st[lane * 33 + e] = v[e0 + e];
+                        for (int e = 0; e < 16; ++e) st[lane * 17 + e] = v[e0 + e];
                         __syncwarp();
-                        const int c = n + e0 + lane;
-                        if (c < p.N)
-                            for (int r = 0; r < 32 && mw + r < p.rows; ++r) {
-                                float y = st[r * 33 + lane];
-                                const int64_t mr = mw + r;
-                                if (p.residual) y += __bfloat162float(p.residual[mr * p.res_stride + c]);
-                                p.out[mr * p.out_stride + c] = __float2bfloat16_rn(y);
-                            }
+                        write_rows<16>(st, p, mw, n + e0, lane);
                         __syncwarp();
                     }
                 }
@@ -501,18 +531,19 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// 2-D row-major [outer][inner] of bf16 or bytes, pitch in elements, boxes of 128 bytes x box_rows, 128-byte swizzle.
-bool encode(CUtensorMap *map, bool bytes, const void *base, int64_t inner, int64_t outer, int64_t pitch, uint32_t box_rows) {
+// 2-D row-major [outer][inner] of bf16 or bytes, pitch in elements; boxes of 128 (or 64) bytes x box_rows, swizzled over their width.
+bool encode(CUtensorMap *map, bool bytes, const void *base, int64_t inner, int64_t outer, int64_t pitch, uint32_t box_rows,
+            int box_bytes = 128) {
     auto fn = encode_fn();
     if (!fn) return false;
     const int es = bytes ? 1 : 2;
     const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
     // with one row the pitch is never used; it must still be a valid one
     const cuuint64_t str[1] = {(cuuint64_t)pitch * es};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / es), box_rows};
+    const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / es), box_rows};
     const cuuint32_t estr[2] = {1, 1};
     return fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base),
-              dims, str, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              dims, str, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -604,18 +635,17 @@ int pair_slots(K kernel, const cudaLaunchConfig_t &cfg, int sms) {
 template <bool E4M3, bool GATED>
 cudaError_t launch_pair(const LinearArgs &a, LinParams p, int sms, cudaStream_t s) {
     constexpr int kOut = GATED ? kPairN / 2 : kPairN;
-    CUtensorMap tx, tw, tg, tres, tout;
+    CUtensorMap tx, tw, tg, tout;
     if (!encode(&tx, E4M3, a.x, a.K, a.rows, a.x_stride, 128)) return cudaErrorInvalidValue;
     if (!encode(&tw, E4M3, a.weight, a.K, a.N, a.K, 128)) return cudaErrorInvalidValue;
-    tg = tres = tout = tw;
+    tg = tout = tw;
     if (GATED && !encode(&tg, E4M3, a.gate, a.K, a.N, a.K, 128)) return cudaErrorInvalidValue;
     auto mappable = [&](const void *ptr, int64_t stride) {
         return a.N % 8 == 0 && stride % 8 == 0 && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0;
     };
     p.tma_out = mappable(a.out, a.out_stride) && (!a.residual || mappable(a.residual, a.res_stride));
-    p.tma_res = p.tma_out && a.residual;
-    if (p.tma_out && !encode(&tout, false, a.out, a.N, a.rows, a.out_stride, 32)) return cudaErrorInvalidValue;
-    if (p.tma_res && !encode(&tres, false, a.residual, a.N, a.rows, a.res_stride, 32)) return cudaErrorInvalidValue;
+    p.vec_res = p.tma_out && a.residual;
+    if (p.tma_out && !encode(&tout, false, a.out, a.N, a.rows, a.out_stride, 32, kEpiCols * 2)) return cudaErrorInvalidValue;
     p.m_tiles = (a.rows + kPairM - 1) / kPairM;
     p.n_tiles = (a.N + kOut - 1) / kOut;
     auto kernel = linear_pair<E4M3, GATED>;
@@ -623,7 +653,7 @@ cudaError_t launch_pair(const LinearArgs &a, LinParams p, int sms, cudaStream_t 
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(2 * (sms / 2)));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kPairThreads);
     cfg.dynamicSmemBytes = kPairSmem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -634,7 +664,7 @@ cudaError_t launch_pair(const LinearArgs &a, LinParams p, int sms, cudaStream_t 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cfg.gridDim = dim3((unsigned)(2 * std::min<long long>((long long)p.m_tiles * p.n_tiles, pair_slots(kernel, cfg, sms))));
-    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, tg, tres, tout, p);
+    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, tg, tout, p);
 }
 
 template <bool E4M3, bool GATED>

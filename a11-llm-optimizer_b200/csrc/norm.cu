@@ -16,10 +16,12 @@
 // reduced together (max|y| = max|h w| * r exactly, since rounding is monotone
 // and y is formed in that order), so the e4m3 output costs no second
 // reduction. Rows of up to 32 vectors belong to one warp (8 rows a block, no
-// block barrier); longer rows to a block of 128 to 1024 threads, wide enough
-// that a thread holds one 16-byte vector where the row allows it (at most 16 values).
-// Rows whose start or length is not a multiple of 16 bytes take the same
-// kernel with one element per access: a warp still covers consecutive bytes.
+// block barrier); longer rows to a block of up to 1024 threads with one to four
+// 16-byte vectors each.
+// Rows of odd length start anywhere, but all tensors' rows at the same distance
+// from a 16-byte boundary: the body is moved in vectors from the first boundary
+// on, and the up to 2 x 7 elements before and after it by one thread each.
+// Where the tensors differ in that distance, every access is one element.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -102,7 +104,8 @@ __device__ __forceinline__ void store_e4m3(uint8_t *p, const float (&f)[VEC]) {
 }
 
 // WARP: a warp per row; otherwise a block per row. NV: vectors a thread holds.
-template <typename T, bool E4M3, int VEC, int NV, bool WARP>
+// PEEL: rows start row * x_stride elements (mod VEC) past a vector boundary.
+template <typename T, bool E4M3, int VEC, int NV, bool WARP, bool PEEL>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) add_rms_norm_kernel(const NormParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
@@ -111,36 +114,52 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) add_rms_norm_kernel(const N
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
     const T *res = p.residual ? static_cast<const T *>(p.residual) + row * p.res_stride : nullptr;
     const T *wt = static_cast<const T *>(p.weight);
+    T *sum = p.sum ? static_cast<T *>(p.sum) + row * p.sum_stride : nullptr;
 
-    float h[NV][VEC];
+    // elements [head, head + body) in vectors; `extra`: this thread's one element of the rest, or -1
+    int head = 0, body = p.dim, extra = -1;
+    if (PEEL) {
+        head = min((int)(-(row * p.x_stride) & (VEC - 1)), p.dim);
+        body = (p.dim - head) & ~(VEC - 1);
+        if (t < head) extra = t;
+        else if (t - head < p.dim - head - body) extra = body + t;
+    }
+    float h[NV][VEC], he = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * threads + t) * VEC;
-        if (c < p.dim) load_vec<T, VEC>(x + c, h[i]);
+        if (c < body) load_vec<T, VEC>(x + head + c, h[i]);
         else
 #pragma unroll
             for (int e = 0; e < VEC; ++e) h[i][e] = 0.0f;
     }
+    if (PEEL && extra >= 0) he = (float)x[extra];
     if (res) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * threads + t) * VEC;
-            if (c < p.dim) {
+            if (c < body) {
                 float r[VEC];
-                load_vec<T, VEC>(res + c, r);
+                load_vec<T, VEC>(res + head + c, r);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) h[i][e] += r[e];
             }
         }
+        if (PEEL && extra >= 0) he += (float)res[extra];
     }
     float ss = 0.0f, mx = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * threads + t) * VEC;
-        if (c < p.dim) {
-            if (p.sum) store_vec<T, VEC>(static_cast<T *>(p.sum) + row * p.sum_stride + c, h[i]);
+        if (c < body) {
+            if (sum) store_vec<T, VEC>(sum + head + c, h[i]);
             float w[VEC];
-            load_vec<T, VEC>(wt + c, w);
+            if constexpr (PEEL) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) w[e] = (float)__ldg(wt + head + c + e);
+            } else {
+                load_vec<T, VEC>(wt + c, w);
+            }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 ss = fmaf(h[i][e], h[i][e], ss);
@@ -148,6 +167,13 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) add_rms_norm_kernel(const N
                 if (E4M3) mx = max_nan(mx, fabsf(h[i][e]));
             }
         }
+    }
+    if (PEEL && extra >= 0) {
+        const float one[1] = {he};
+        if (sum) store_vec<T, 1>(sum + extra, one);
+        ss = fmaf(he, he, ss);
+        he *= (float)__ldg(wt + extra);
+        if (E4M3) mx = max_nan(mx, fabsf(he));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -175,44 +201,54 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) add_rms_norm_kernel(const N
         inv = 1.0f / scale;
         if (t == 0) p.scales[row] = scale;
     }
+    auto put = [&](int c, auto &v) {  // v: VEC or one elements at c
+        constexpr int W = sizeof(v) / sizeof(float);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+            v[e] *= r;
+            if (E4M3) v[e] *= inv;
+        }
+        if constexpr (E4M3) store_e4m3<W>(static_cast<uint8_t *>(p.out) + row * p.out_stride + c, v);
+        else store_vec<T, W>(static_cast<T *>(p.out) + row * p.out_stride + c, v);
+    };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * threads + t) * VEC;
-        if (c < p.dim) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                h[i][e] *= r;
-                if (E4M3) h[i][e] *= inv;
-            }
-            if constexpr (E4M3) store_e4m3<VEC>(static_cast<uint8_t *>(p.out) + row * p.out_stride + c, h[i]);
-            else store_vec<T, VEC>(static_cast<T *>(p.out) + row * p.out_stride + c, h[i]);
-        }
+        if (c < body) put(head + c, h[i]);
+    }
+    if (PEEL && extra >= 0) {
+        float one[1] = {he};
+        put(extra, one);
     }
 }
 
-template <typename T, bool E4M3, int VEC>
+template <typename T, bool E4M3, int VEC, bool PEEL>
 cudaError_t launch_vec(const NormParams &p, cudaStream_t s) {
     // values a thread holds: one vector (8 single elements) while 1024 threads
-    // cover the row, else 16 (A11S_NORM_MAX_DIM = 1024 * 16)
+    // cover the row that way, else up to 16 (A11S_NORM_MAX_DIM = 1024 * 16).
+    // Holding two or four vectors in fewer threads measured the same at
+    // 2048 x 2048 and 1 x 2048 (within 2 %).
     constexpr int kFirst = VEC == 1 ? 8 : 1, kLast = 16 / VEC;
     const int vecs = (p.dim + VEC - 1) / VEC;
     if (vecs <= 32 * kFirst) {
-        add_rms_norm_kernel<T, E4M3, VEC, kFirst, true><<<(unsigned)((p.rows + 7ll) / 8), 256, 0, s>>>(p);
+        add_rms_norm_kernel<T, E4M3, VEC, kFirst, true, PEEL><<<(unsigned)((p.rows + 7ll) / 8), 256, 0, s>>>(p);
         return cudaGetLastError();
     }
-    int threads = 128;
-    while (threads < 1024 && threads * kFirst < vecs) threads *= 2;
-    const int nv = (vecs + threads - 1) / threads;
-    if (nv <= kFirst) add_rms_norm_kernel<T, E4M3, VEC, kFirst, false><<<(unsigned)p.rows, threads, 0, s>>>(p);
-    else if (nv <= 2 * kFirst) add_rms_norm_kernel<T, E4M3, VEC, 2 * kFirst, false><<<(unsigned)p.rows, threads, 0, s>>>(p);
-    else if (nv <= kLast) add_rms_norm_kernel<T, E4M3, VEC, kLast, false><<<(unsigned)p.rows, threads, 0, s>>>(p);
+    int nv = kFirst;
+    while (vecs > 1024 * nv) nv *= 2;
+    const int threads = ((vecs + nv - 1) / nv + 31) / 32 * 32;
+    if (nv == kFirst) add_rms_norm_kernel<T, E4M3, VEC, kFirst, false, PEEL><<<(unsigned)p.rows, threads, 0, s>>>(p);
+    else if (nv == 2 * kFirst) add_rms_norm_kernel<T, E4M3, VEC, 2 * kFirst, false, PEEL><<<(unsigned)p.rows, threads, 0, s>>>(p);
+    else if (nv <= kLast) add_rms_norm_kernel<T, E4M3, VEC, kLast, false, PEEL><<<(unsigned)p.rows, threads, 0, s>>>(p);
     else return cudaErrorInvalidValue;
     return cudaGetLastError();
 }
 
 template <typename T, bool E4M3>
-cudaError_t launch_type(const NormParams &p, bool vec, cudaStream_t s) {
-    return vec ? launch_vec<T, E4M3, 16 / (int)sizeof(T)>(p, s) : launch_vec<T, E4M3, 1>(p, s);
+cudaError_t launch_type(const NormParams &p, int vec, cudaStream_t s) {
+    constexpr int kVec = 16 / (int)sizeof(T);
+    if (vec == 2) return launch_vec<T, E4M3, kVec, false>(p, s);
+    return vec == 1 ? launch_vec<T, E4M3, kVec, true>(p, s) : launch_vec<T, E4M3, 1, false>(p, s);
 }
 }  // namespace
 
@@ -232,12 +268,14 @@ cudaError_t launch_add_rms_norm(const NormArgs &a, cudaStream_t s) {
     p.dim = a.dim;
     p.eps = a.eps;
     const int es = a.bf16 ? 2 : 4, os = a.e4m3 ? 1 : es, per = 16 / es;
-    auto ok = [](const void *ptr, int64_t stride, int size, int bytes) {
-        return (reinterpret_cast<uintptr_t>(ptr) % bytes) == 0 && (stride * size) % bytes == 0;
-    };
-    const bool vec = a.dim % per == 0 && ok(a.x, a.x_stride, es, 16) && ok(a.residual, a.res_stride, es, 16) &&
-                     ok(a.weight, 0, es, 16) && ok(a.sum, a.sum_stride, es, 16) &&
-                     ok(a.out, a.out_stride, os, per * os);
+    // 2: rows and lengths in whole vectors; 1: rows of every tensor equally far past a vector boundary; 0: neither
+    auto base = [](const void *ptr, int bytes) { return (reinterpret_cast<uintptr_t>(ptr) % bytes) == 0; };
+    int vec = 0;
+    if (base(a.x, 16) && base(a.residual, 16) && base(a.weight, 16) && base(a.sum, 16) && base(a.out, per * os)) {
+        const int64_t d = a.x_stride % per;
+        if (a.out_stride % per == d && (!a.residual || a.res_stride % per == d) && (!a.sum || a.sum_stride % per == d))
+            vec = d == 0 && a.dim % per == 0 ? 2 : 1;
+    }
     if (a.bf16)
         return a.e4m3 ? launch_type<__nv_bfloat16, true>(p, vec, s) : launch_type<__nv_bfloat16, false>(p, vec, s);
     return a.e4m3 ? launch_type<float, true>(p, vec, s) : launch_type<float, false>(p, vec, s);

@@ -102,13 +102,16 @@ def test_row_strides():
 
     class Fake:  # a CPU view that says it is on the device
         def __init__(self, t):
-            self.t, self.is_cuda, self.device = t, True, "dev"
+            self.t = t
+
+        def get_device(self):
+            return 0
 
         def __getattr__(self, k):
             return getattr(self.t, k)
 
     t = torch.zeros(4, 6, 3, 136, dtype=torch.bfloat16)
-    f = lambda v, d: _rows(Fake(v), "x", d, torch.bfloat16, "dev")  # noqa: E731
+    f = lambda v, d: _rows(Fake(v), "x", d, torch.bfloat16, 0)  # noqa: E731
     assert f(t, 136) == 136 and f(t[:, :, 1, :128], 128) == 408 and f(t[:, :1, 1, :128], 128) == 6 * 408
     assert f(t[:1, :1, :1, :128], 128) == 128 and f(t[0, 0, 0, :8], 8) == 8 and f(t[:0], 136) == 136
     for v in (t[:, 1:3, 1], t.transpose(0, 1)[..., :128], t[..., ::2], t[0, 0, 0, ::2]):
