@@ -580,13 +580,32 @@ int a11s_tree_attention(const void *q, const void *k_pool, const void *v_pool, i
 }
 
 // ------------------------------------------------------------------- K10
+namespace {
+// Workspace: status word and (few rows) the merge counters, cleared before each
+// launch, then partial outputs and partial (maximum, sum) pairs.
+struct ChunkLayout {
+    size_t part_o, part_ml, total;
+};
+ChunkLayout chunk_layout(const a11s::ChunkPlan &plan, int32_t batch, int32_t max_new, int32_t num_q_heads, int32_t num_kv_heads,
+                         int32_t head_dim) {
+    ChunkLayout l;
+    l.part_o = kHeaderBytes + (plan.rows ? up256((size_t)batch * num_kv_heads * sizeof(int32_t)) : 0);
+    const size_t rows = plan.rows ? (size_t)2 * plan.splits * ((max_new * (num_q_heads / num_kv_heads) + 7) / 8 * 8)
+                        : plan.splits > 1 ? (size_t)plan.splits * batch * max_new * num_q_heads : 0;
+    l.part_ml = l.part_o + up256(rows * head_dim * sizeof(float));
+    l.total = l.part_ml + up256(rows * 2 * sizeof(float));
+    return l;
+}
+}  // namespace
+
 size_t a11s_chunk_attention_workspace_bytes(int32_t batch, int32_t max_new, int32_t num_q_heads,
                                             int32_t num_kv_heads, int32_t head_dim, int32_t max_kv_len) {
     if (batch < 0 || max_new < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || num_q_heads / num_kv_heads > 128 ||
         head_dim < 1 || max_kv_len < 1)
         return 0;
+    if (batch == 0) return kHeaderBytes;
     const a11s::ChunkPlan plan = a11s::chunk_attention_plan(batch, max_new, num_q_heads, num_kv_heads, max_kv_len);
-    return kHeaderBytes + up256(a11s::chunk_attention_partials_bytes(batch, max_new, num_q_heads, head_dim, plan.splits));
+    return chunk_layout(plan, batch, max_new, num_q_heads, num_kv_heads, head_dim).total;
 }
 
 int a11s_chunk_attention(const void *q, int64_t q_stride, const void *k_pool, const void *v_pool, int32_t num_pages,
@@ -615,8 +634,8 @@ int a11s_chunk_attention(const void *q, int64_t q_stride, const void *k_pool, co
         return fail(A11S_EINVAL, "a11s_chunk_attention: tensors must be 16-byte aligned");
     a11s::ChunkAttnArgs a{};
     a.plan = a11s::chunk_attention_plan(batch, max_new, num_q_heads, num_kv_heads, max_kv_len);
-    const size_t need = kHeaderBytes + up256(a11s::chunk_attention_partials_bytes(batch, max_new, num_q_heads, head_dim,
-                                                                                  a.plan.splits));
+    const ChunkLayout lay = chunk_layout(a.plan, batch, max_new, num_q_heads, num_kv_heads, head_dim);
+    const size_t need = lay.total;
     if (workspace_bytes < need)
         return fail(A11S_ENOSPACE, "a11s_chunk_attention: workspace %zu < %zu bytes", workspace_bytes, need);
     if ((double)a.plan.ctiles * batch * a.plan.splits * num_kv_heads > 2147483647.0 ||
@@ -641,10 +660,11 @@ int a11s_chunk_attention(const void *q, int64_t q_stride, const void *k_pool, co
     a.lse = lse;
     char *ws = static_cast<char *>(workspace);
     a.status = reinterpret_cast<a11s::StatusWord *>(ws);
-    a.part_o = reinterpret_cast<float *>(ws + kHeaderBytes);
-    a.part_ml = a.part_o + (size_t)a.plan.splits * batch * max_new * num_q_heads * head_dim;
+    a.counters = reinterpret_cast<int32_t *>(ws + kHeaderBytes);
+    a.part_o = reinterpret_cast<float *>(ws + lay.part_o);
+    a.part_ml = reinterpret_cast<float *>(ws + lay.part_ml);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(a11s::StatusWord), s);
+    cudaError_t e = cudaMemsetAsync(ws, 0, a.plan.rows ? lay.part_o : sizeof(a11s::StatusWord), s);
     if (e != cudaSuccess) return cuda_fail(e, "a11s_chunk_attention: clearing status");
     e = a11s::launch_chunk_attention(a, s);
     if (e != cudaSuccess) return cuda_fail(e, "a11s_chunk_attention: launch");

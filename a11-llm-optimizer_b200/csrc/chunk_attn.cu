@@ -545,9 +545,15 @@ __global__ void __launch_bounds__(D) chunk_attn_combine(const Params p) {
 
 // ---------------------------------------------------------------------------- host side
 ChunkPlan chunk_attention_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t max_kv_len) {
+    const int max_pages = (max_kv_len + A11S_PAGE_TOKENS - 1) / A11S_PAGE_TOKENS;
     int sms = 148, dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     ChunkPlan c;
+    if ((long long)N * (Hq / Hkv) <= kChunkRows && B <= kChunkRowsMaxBatch && (double)B * Hkv * max_pages < 1e9) {
+        c.rows = true;
+        c.splits = chunk_rows_ctas(sms);
+        return c;
+    }
     c.tokens = 128 / (Hq / Hkv);
     c.ctiles = (N + kTiles * c.tokens - 1) / (kTiles * c.tokens);
     const long long ctas = (long long)B * Hkv * c.ctiles;
@@ -569,10 +575,6 @@ ChunkPlan chunk_attention_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, in
     c.split_blocks = (blocks + c.splits - 1) / c.splits;
     c.splits = (blocks + c.split_blocks - 1) / c.split_blocks;
     return c;
-}
-
-size_t chunk_attention_partials_bytes(int32_t B, int32_t N, int32_t Hq, int32_t D, int32_t splits) {
-    return splits > 1 ? (size_t)splits * B * N * Hq * (D + 2) * sizeof(float) : 0;
 }
 
 namespace {
@@ -623,6 +625,7 @@ cudaError_t launch_d(const ChunkAttnArgs &a, const Params &p, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_chunk_attention(const ChunkAttnArgs &a, cudaStream_t s) {
+    if (a.plan.rows) return launch_chunk_attention_rows(a, s);
     Params p{};
     p.q = reinterpret_cast<const __nv_bfloat16 *>(a.q);
     p.q_stride = a.q_stride;

@@ -6,7 +6,27 @@
 namespace a11s {
 
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
-__device__ __forceinline__ float gelu(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f)); }
+// v Phi(v) with Phi(-|v|) = exp(-v^2 / 2) erfcx(|v| / sqrt(2)) / 2, where erfcx(z) =
+// exp(z^2) erfc(z) is a polynomial in t = 1 / (1 + 0.38 z) (the form of Hastings'
+// approximations; own least-squares fit, reweighted towards the least relative
+// error: 2.2e-8 on [0, 12]). Without branches, so that the columns of a step run
+// side by side: erff, with its two ranges, took 300 cycles a column in a warp
+// that has its scheduler to itself. Relative error in fp32 below 1.0e-6 for v > -4
+// and 2.1e-6 down to -6, where v Phi(v) is 6e-9.
+__device__ __forceinline__ float gelu(float v) {
+    const float t = __fdividef(1.0f, fmaf(0.26870057f, fabsf(v), 1.0f));
+    float r = 0.0590475053f;
+    r = fmaf(r, t, -0.262688488f);
+    r = fmaf(r, t, 0.364739329f);
+    r = fmaf(r, t, -0.162510931f);
+    r = fmaf(r, t, 0.230789483f);
+    r = fmaf(r, t, 0.138305649f);
+    r = fmaf(r, t, 0.204000324f);
+    r = fmaf(r, t, 0.213905275f);
+    r = fmaf(r, t, 0.214411855f);
+    const float q = 0.5f * t * r * exp2f(v * v * -0.72134752f);
+    return v * (v < 0.0f ? q : 1.0f - q);
+}
 
 __device__ __forceinline__ float activate(float v, int act) {
     return act == A11S_ACT_SILU ? silu(v) : act == A11S_ACT_GELU ? gelu(v) : v;

@@ -165,12 +165,16 @@ struct AttnArgs {
 cudaError_t launch_tree_attention(const AttnArgs &a, cudaStream_t s);
 
 // How a11s_chunk_attention cuts its work: tokens of a Q tile, CTAs along the
-// chunk, and at most `splits` splits of `split_blocks` 128-key blocks along the cache.
+// chunk, and at most `splits` splits of `split_blocks` 128-key blocks along the
+// cache. rows: few query rows (chunk_attn_rows.cu), splits counts its CTAs.
 struct ChunkPlan {
     int32_t tokens = 1, ctiles = 1, splits = 1, split_blocks = 1;
+    bool rows = false;
 };
+constexpr int kChunkRows = 32;            // tokens x query heads of a KV head up to which the cache is streamed by warps
+constexpr int kChunkRowsMaxBatch = 2048;  // its page sums fit shared memory
+int chunk_rows_ctas(int sms);
 ChunkPlan chunk_attention_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t max_kv_len);
-size_t chunk_attention_partials_bytes(int32_t B, int32_t N, int32_t Hq, int32_t D, int32_t splits);
 
 struct ChunkAttnArgs {
     const void *q, *k_pool, *v_pool;
@@ -183,10 +187,13 @@ struct ChunkAttnArgs {
     float scale;
     void *out;
     float *lse;               // nullable
-    float *part_o, *part_ml;  // [splits][B][N][Hq][D], [splits][B][N][Hq][2] (reference maximum in log2 units, sum)
+    float *part_o, *part_ml;  // [splits][B][N][Hq][D], [splits][B][N][Hq][2] (reference maximum in log2 units,
+                              // sum); few rows: chunk_attn_rows.cu
+    int32_t *counters;        // [B][Hkv] (few rows), zero at the launch
     ChunkPlan plan;
     StatusWord *status;
 };
+cudaError_t launch_chunk_attention_rows(const ChunkAttnArgs &a, cudaStream_t s);
 cudaError_t launch_chunk_attention(const ChunkAttnArgs &a, cudaStream_t s);
 
 struct NormArgs {

@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 
 #include "epilogue.cuh"
 #include "kernels.h"
@@ -50,6 +51,7 @@ struct LinParams {
     __nv_bfloat16 *out;
     int64_t res_stride, out_stride;
     int32_t rows, N, act, m_tiles, n_tiles, slices, split;
+    int32_t vec4;              // linear_tile: out and residual rows take 8-byte accesses, N a multiple of 4
     int32_t tma_out, vec_res;  // linear_pair: out takes a tensor map; residual rows are read 16 bytes at a time
     StatusWord *status;
 };
@@ -79,10 +81,10 @@ constexpr uint32_t kTileABytes = kTileM * kSliceBytes;  // 16 KB
 template <int BN>
 struct TileShape {
     static constexpr uint32_t kStage = kTileABytes + BN * kSliceBytes;
-    static constexpr int kStages = BN == 64 ? 8 : 6;
-    static constexpr uint32_t kRing = kStages * kStage;  // 192 KB
-    static constexpr uint32_t kOffCols = kRing;       // 4 x 128 column parameters
-    static constexpr uint32_t kOffBars = kRing + 2048;
+    static constexpr int kStages = BN == 128 ? 6 : 8;
+    static constexpr uint32_t kRing = kStages * kStage;  // 160 to 192 KB
+    static constexpr uint32_t kOffCols = kRing;       // 4 x 128 column parameters, 128 row scales
+    static constexpr uint32_t kOffBars = kRing + 2560;
     static constexpr uint32_t kSmem = kOffBars + 512 + 1024;
 };
 struct TileBars : BarsCommon {
@@ -101,16 +103,105 @@ __device__ __forceinline__ void epilogue_barrier() {
 template <int C>
 __device__ __forceinline__ void write_rows(const float *stage, const LinParams &p, int m0, int n0, int lane) {
     constexpr int kRows = C >= 32 ? 1 : 32 / C, kParts = C >= 32 ? C / 32 : 1;  // rows per access, accesses per row
+    constexpr int kSteps = 32 / kRows * kParts, kBatch = kSteps < 8 ? kSteps : kSteps <= 16 ? 8 : 16;
     const int r0 = C >= 32 ? 0 : lane / C, c0 = C >= 32 ? lane : lane % C;
-#pragma unroll 8
-    for (int i = 0; i < 32 / kRows * kParts; ++i) {
-        const int r = i / kParts * kRows + r0, c = c0 + (i % kParts) * 32;
-        const int64_t m = m0 + r;
-        const int n = n0 + c;
-        if (m < p.rows && n < p.N) {
-            float y = stage[r * (C + 1) + c];
-            if (p.residual) y += __bfloat162float(p.residual[m * p.res_stride + n]);
-            p.out[m * p.out_stride + n] = __float2bfloat16_rn(y);
+#pragma unroll 1
+    for (int i0 = 0; i0 < kSteps; i0 += kBatch) {
+        // all of a batch's residual loads (absent elements: the last one again) before
+        // its stores, since out may be the residual
+        __nv_bfloat16 res[kBatch];
+        if (p.residual) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int r = (i0 + i) / kParts * kRows + r0, c = c0 + (i0 + i) % kParts * 32;
+                res[i] = p.residual[(int64_t)min(m0 + r, p.rows - 1) * p.res_stride + min(n0 + c, p.N - 1)];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) res[i] = __float2bfloat16_rn(0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int r = (i0 + i) / kParts * kRows + r0, c = c0 + (i0 + i) % kParts * 32;
+            const float y = stage[r * (C + 1) + c] + __bfloat162float(res[i]);
+            if (m0 + r < p.rows && n0 + c < p.N) p.out[(int64_t)(m0 + r) * p.out_stride + n0 + c] = __float2bfloat16_rn(y);
+        }
+    }
+}
+
+// This CTA's share (kOut / SPLIT columns) of the tile: the sums of the cluster's
+// CTAs, added in rank order, finished and written by the 128 epilogue threads t.
+// A thread takes four columns of every kPer-th group of rows, so that a warp's
+// loads from the other CTAs run along rows (whole lines: with a row per lane they
+// took 2400 cycles a step) and its columns' parameters stay in registers.
+template <bool GATED, int kOut, int SPLIT>
+__device__ __forceinline__ void merge_split(const float *part, const float *cols_sm, const float *xs_sm, const LinParams &p,
+                                            int rank, int t, int m0, int n0, bool params) {
+    constexpr int kCols = kOut / SPLIT, kPer = kCols / 4, kStep = kTileM / kPer;  // threads of a row, rows of a pass
+    constexpr int kPitch = (GATED ? 2 * kOut : kOut) + 4;
+    constexpr int kBatch = kPer < 2 ? 1 : SPLIT * (GATED ? 2 : 1) <= 8 && kPer >= 4 ? 4 : 2;  // passes in flight
+    const int c = rank * kCols + t % kPer * 4, r0 = t / kPer, n = n0 + c;
+    float4 ws = make_float4(1, 1, 1, 1), wb = make_float4(0, 0, 0, 0), gs = ws, gb = wb;
+    if (params) {
+        ws = *reinterpret_cast<const float4 *>(cols_sm + c);
+        wb = *reinterpret_cast<const float4 *>(cols_sm + kOut + c);
+        if constexpr (GATED) {
+            gs = *reinterpret_cast<const float4 *>(cols_sm + 2 * kOut + c);
+            gb = *reinterpret_cast<const float4 *>(cols_sm + 3 * kOut + c);
+        }
+    }
+    uint32_t src[SPLIT];
+#pragma unroll
+    for (int r = 0; r < SPLIT; ++r) src[r] = tc::cluster_addr(part, r) + (uint32_t)(r0 * kPitch + c) * 4;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kPer; i0 += kBatch) {
+        float4 a[kBatch][SPLIT], g[GATED ? kBatch : 1][GATED ? SPLIT : 1], res[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+#pragma unroll
+            for (int r = 0; r < SPLIT; ++r) {
+                const uint32_t at = src[r] + (uint32_t)((i0 + i) * kStep * kPitch) * 4;
+                a[i][r] = tc::ld_cluster_v4(at + (GATED ? kOut * 4 : 0));
+                if constexpr (GATED) g[i][r] = tc::ld_cluster_v4(at);
+            }
+            res[i] = make_float4(0, 0, 0, 0);
+            if (p.residual) {  // absent elements: the last ones again
+                const __nv_bfloat16 *row = p.residual + (int64_t)min(m0 + r0 + (i0 + i) * kStep, p.rows - 1) * p.res_stride;
+                if (p.vec4) {
+                    const uint2 w = *reinterpret_cast<const uint2 *>(row + min(n, p.N - 4));
+                    res[i] = make_float4(bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y));
+                } else {
+                    res[i] = make_float4(__bfloat162float(row[min(n, p.N - 1)]), __bfloat162float(row[min(n + 1, p.N - 1)]),
+                                         __bfloat162float(row[min(n + 2, p.N - 1)]), __bfloat162float(row[min(n + 3, p.N - 1)]));
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int row = r0 + (i0 + i) * kStep, m = m0 + row;
+            const float xs = params ? xs_sm[row] : 1.0f;
+            float4 v = a[i][0], u = make_float4(0, 0, 0, 0);
+            if constexpr (GATED) u = g[i][0];
+#pragma unroll
+            for (int r = 1; r < SPLIT; ++r) {
+                v = make_float4(v.x + a[i][r].x, v.y + a[i][r].y, v.z + a[i][r].z, v.w + a[i][r].w);
+                if constexpr (GATED) u = make_float4(u.x + g[i][r].x, u.y + g[i][r].y, u.z + g[i][r].z, u.w + g[i][r].w);
+            }
+            const float y0 = finish<GATED>(v.x, u.x, xs, Column{ws.x, wb.x, gs.x, gb.x}, p.act) + res[i].x;
+            const float y1 = finish<GATED>(v.y, u.y, xs, Column{ws.y, wb.y, gs.y, gb.y}, p.act) + res[i].y;
+            const float y2 = finish<GATED>(v.z, u.z, xs, Column{ws.z, wb.z, gs.z, gb.z}, p.act) + res[i].z;
+            const float y3 = finish<GATED>(v.w, u.w, xs, Column{ws.w, wb.w, gs.w, gb.w}, p.act) + res[i].w;
+            if (m < p.rows) {
+                __nv_bfloat16 *o = p.out + (int64_t)m * p.out_stride + n;
+                if (p.vec4) {
+                    if (n < p.N) *reinterpret_cast<uint2 *>(o) = make_uint2(tc::cvt_bf16x2(y0, y1), tc::cvt_bf16x2(y2, y3));
+                } else {
+                    if (n < p.N) o[0] = __float2bfloat16_rn(y0);
+                    if (n + 1 < p.N) o[1] = __float2bfloat16_rn(y1);
+                    if (n + 2 < p.N) o[2] = __float2bfloat16_rn(y2);
+                    if (n + 3 < p.N) o[3] = __float2bfloat16_rn(y3);
+                }
+            }
         }
     }
 }
@@ -154,6 +245,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
         if (lane == 0) {
             constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
+            tc::prefetch_tmap(&tx);
+            tc::prefetch_tmap(&tw);
+            if (GATED) tc::prefetch_tmap(&tg);
             for (int i = 0; i < ns; ++i) {
                 const int s = i % S::kStages, use = i / S::kStages;
                 if (use > 0 && !wait_or_abort(&bs->empty[s], (use - 1) & 1, bs, p.status)) break;
@@ -197,33 +291,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- epilogue warps ----------------
     const int q = warp & 3, row = q * 32 + lane, m = m0 + row;  // TMEM lane = tile row
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
-    float *cols_sm = reinterpret_cast<float *>(sm + S::kOffCols);
+    float *cols_sm = reinterpret_cast<float *>(sm + S::kOffCols), *xs_sm = cols_sm + 512;
     const bool params = p.col.any();
     float xs = 1.0f;
     bool ok = true;
     if (warp >= 2) {
         if (params) stage_columns<GATED, kOut>(cols_sm, p.col, n0, p.N, threadIdx.x - 64, 128);
         if (E4M3 && m < p.rows) xs = __ldg(p.x_scale + m);
+        if (params) xs_sm[row] = xs;
         epilogue_barrier<128>();
         ok = __all_sync(0xffffffffu, wait_or_abort(&bs->acc_full, 0, bs, p.status));
         tc::tc_fence_after();
     }
     // With the accumulator complete the ring is free. part: this CTA's sums,
-    // [BN][128] fp32, column-major; stage: finished outputs of an epilogue warp.
+    // [128][BN + 4] fp32; stage: finished outputs of an epilogue warp.
     float *part = reinterpret_cast<float *>(sm);
-    float *stage = reinterpret_cast<float *>(sm + BN * kTileM * 4) + q * 32 * (kOut + 1);
+    float *stage = part + kTileM * (BN + 4) + q * 32 * (kOut + 1);
     if (p.split == 1) {
+        constexpr int kW = kOut < 32 ? kOut : 32;
         if (warp >= 2 && ok) {
 #pragma unroll 1
-            for (int c = 0; c < kOut; c += 32) {
-                float v[32], u[GATED ? 32 : 1];
-                tc::tmem_ld32(tmem + lane_base + (GATED ? kOut : 0) + c, v);
-                if constexpr (GATED) tc::tmem_ld32(tmem + lane_base + c, u);
+            for (int c = 0; c < kOut; c += kW) {
+                float v[kW], u[GATED ? kW : 1];
+                if constexpr (kW == 32) {
+                    tc::tmem_ld32(tmem + lane_base + (GATED ? kOut : 0) + c, v);
+                    if constexpr (GATED) tc::tmem_ld32(tmem + lane_base + c, u);
+                } else {  // gate and weight columns side by side
+                    float both[32];
+                    tc::tmem_ld32(tmem + lane_base, both);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        u[e] = both[e];
+                        v[e] = both[16 + e];
+                    }
+                }
                 finish_columns<GATED, kOut>(v, u, xs, cols_sm, c, params, p.act);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) stage[lane * 33 + e] = v[e];
+                for (int e = 0; e < kW; ++e) stage[lane * (kW + 1) + e] = v[e];
                 __syncwarp();
-                write_rows<32>(stage, p, m0 + q * 32, n0 + c, lane);
+                write_rows<kW>(stage, p, m0 + q * 32, n0 + c, lane);
                 __syncwarp();
             }
         }
@@ -239,41 +345,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int e = 0; e < 32; ++e) v[e] = 0.0f;
                 }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) part[(c + e) * kTileM + row] = v[e];
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<float4 *>(part + row * (BN + 4) + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
             }
         }
         __syncwarp();
         tc::cluster_sync();  // every CTA's sums are in shared memory (and after a timeout nobody waits for them)
         if (warp >= 2 && ok) {
-            const int cols = kOut / p.split, c0 = rank * cols;  // this CTA's output columns of the tile
-            uint32_t src[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) src[r] = tc::cluster_addr(part, r < p.split ? r : 0) + (uint32_t)row * 4;
-#pragma unroll 1
-            for (int c = 0; c < cols; c += 4) {
-                // gated: the gate's columns are the first half of the tile
-                float v[4] = {}, u[4] = {};
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (r < p.split) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            v[e] += tc::ld_cluster_f32(src[r] + ((GATED ? kOut : 0) + c0 + c + e) * (kTileM * 4));
-                            if (GATED) u[e] += tc::ld_cluster_f32(src[r] + (c0 + c + e) * (kTileM * 4));
-                        }
-                    }
-                finish_columns<GATED, kOut>(v, u, xs, cols_sm, c0 + c, params, p.act);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) stage[lane * (cols + 1) + c + e] = v[e];
-            }
-            __syncwarp();
-            switch (cols) {
-                case 4: write_rows<4>(stage, p, m0 + q * 32, n0 + c0, lane); break;
-                case 8: write_rows<8>(stage, p, m0 + q * 32, n0 + c0, lane); break;
-                case 16: write_rows<16>(stage, p, m0 + q * 32, n0 + c0, lane); break;
-                case 32: write_rows<32>(stage, p, m0 + q * 32, n0 + c0, lane); break;
-                default: write_rows<64>(stage, p, m0 + q * 32, n0 + c0, lane); break;
-            }
+            auto merge = [&](auto split) {
+                merge_split<GATED, kOut, decltype(split)::value>(part, cols_sm, xs_sm, p, rank, threadIdx.x - 64, m0, n0, params);
+            };
+            if (p.split == 2) merge(std::integral_constant<int, 2>{});
+            else if (p.split == 4) merge(std::integral_constant<int, 4>{});
+            else if constexpr (kOut >= 32) merge(std::integral_constant<int, 8>{});
         }
     }
     // After a timeout copies may still be landing here: give them time (about
@@ -575,13 +659,13 @@ Plan choose(const LinearArgs &a, int slices, int sms) {
         const double waves = (double)((t + sms / 2 - 1) / (sms / 2));
         best.cost = waves * (slices * 540.0) + 5000.0;
     }
-    for (int bn : {64, 128})
+    for (int bn : {32, 64, 128})
         for (int split : {1, 2, 4, 8}) {
-            if (split > 1 && split > slices) break;
+            if (split > 1 && (split > slices || (bn == 32 && a.gate && split == 8))) break;
             const long long t = tiles(kTileM, a.gate ? bn / 2 : bn) * split;
             const double waves = (double)((t + sms - 1) / sms);
             const double per = (slices + split - 1) / split;
-            const double cost = waves * (per * (bn == 64 ? 400.0 : 540.0) + 3500.0 + (split > 1 ? 1500.0 : 0.0));
+            const double cost = waves * (per * (bn == 32 ? 340.0 : bn == 64 ? 400.0 : 540.0) + 3500.0 + (split > 1 ? 1500.0 : 0.0));
             if (cost < best.cost) {
                 best.cost = cost;
                 best.bn = bn;
@@ -602,6 +686,10 @@ cudaError_t launch_tile(const LinearArgs &a, LinParams p, int split, cudaStream_
     p.m_tiles = (a.rows + kTileM - 1) / kTileM;
     p.n_tiles = (a.N + kOut - 1) / kOut;
     p.split = split;
+    auto vec4 = [&](const void *ptr, int64_t stride) {
+        return a.N % 4 == 0 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(ptr) & 7) == 0;
+    };
+    p.vec4 = vec4(a.out, a.out_stride) && (!a.residual || vec4(a.residual, a.res_stride));
     auto kernel = linear_tile<E4M3, GATED, BN>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<BN>::kSmem);
     if (e != cudaSuccess) return e;
@@ -685,8 +773,11 @@ cudaError_t launch_type(const LinearArgs &a, cudaStream_t s) {
     const int sms = device_sms();
     const Plan plan = choose(a, p.slices, sms);
     if (plan.bn == 0) return launch_pair<E4M3, GATED>(a, p, sms, s);
-    return plan.bn == 64 ? launch_tile<E4M3, GATED, 64>(a, p, plan.split, s)
-                         : launch_tile<E4M3, GATED, 128>(a, p, plan.split, s);
+    switch (plan.bn) {
+        case 32: return launch_tile<E4M3, GATED, 32>(a, p, plan.split, s);
+        case 64: return launch_tile<E4M3, GATED, 64>(a, p, plan.split, s);
+        default: return launch_tile<E4M3, GATED, 128>(a, p, plan.split, s);
+    }
 }
 }  // namespace
 

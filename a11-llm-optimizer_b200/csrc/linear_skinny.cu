@@ -19,6 +19,7 @@
 
 #include "epilogue.cuh"
 #include "kernels.h"
+#include "mma_sync.cuh"
 
 namespace a11s {
 namespace {
@@ -34,17 +35,6 @@ struct SkinnyParams {
     StatusWord *status;
 };
 
-template <bool E4M3>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (E4M3)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 // Four e4m3 values as two f16 pairs (exact).
 __device__ __forceinline__ void widen(uint32_t v, uint32_t &lo, uint32_t &hi) {
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
@@ -63,13 +53,13 @@ __device__ __forceinline__ void product16(float (&d)[4], const uint4 &w0, const 
             widen(p[i], a[0], a[2]);
             widen(q[i], a[1], a[3]);
             widen(b[i], b0, b1);
-            mma16816<true>(d, a, b0, b1);
+            mma16816_f16(d, a, b0, b1);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
             const uint32_t a[4] = {p[i], q[i], p[i + 1], q[i + 1]};
-            mma16816<false>(d, a, b[i], b[i + 1]);
+            mma16816_bf16(d, a, b[i], b[i + 1]);
         }
     }
 }

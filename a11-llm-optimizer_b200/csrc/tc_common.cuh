@@ -178,10 +178,13 @@ __device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(p)), "r"(rank));
     return d;
 }
-// fp32 of another CTA's shared memory (shared::cluster address).
-__device__ __forceinline__ float ld_cluster_f32(uint32_t caddr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(caddr) : "memory");
+// Four fp32 of another CTA's shared memory (shared::cluster address).
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t caddr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(caddr)
+                 : "memory");
     return v;
 }
 // Arrive once on an mbarrier given by its shared::cluster address (this CTA's or the peer's).
