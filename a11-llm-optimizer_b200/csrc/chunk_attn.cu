@@ -105,6 +105,10 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, Ba
     report(st, A11S_ETIMEOUT, 0);
     return false;
 }
+// The same by a whole warp, with one answer for all its lanes (a converged warp stays one).
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, Bars *bs, StatusWord *st) {
+    return __all_sync(0xffffffffu, wait_or_abort(bar, parity, bs, st));
+}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -267,42 +271,50 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == kMmaWarp) {
             // ---------------- S issuer ----------------
-            if (lane == 0) {
-                constexpr uint32_t idesc = tc::idesc_bf16_f32(128, kBlockKV, false);
-                bool ok = wait_or_abort(&bs->q_ready, 0, bs, p.status);
-                int u = 0;
-                for (int j = 0; j < nb && ok; ++j) {
-                    for (int t = 0; t < nt; ++t, ++u) {
-                        if (u > 0) ok = wait_or_abort(&bs->s_free, (u - 1) & 1, bs, p.status);
-                        if (ok && t == 0) ok = wait_or_abort(&bs->k_full[j % S::kKStages], (j / S::kKStages) & 1, bs, p.status);
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        const uint32_t k_addr = tc::smem_u32(sm + S::kOffK + (j % S::kKStages) * S::kSlot);
-                        const uint32_t q_addr = tc::smem_u32(sm + t * S::kQTile);
+            constexpr uint32_t idesc = tc::idesc_bf16_f32(128, kBlockKV, false);
+            const uint64_t qd0 = tc::sdesc_sw128(tc::smem_u32(sm), 16, 1024), kd0 = tc::sdesc_sw128(tc::smem_u32(sm + S::kOffK), 16, 1024);
+            bool ok = warp_wait(&bs->q_ready, 0, bs, p.status);
+            int ks = 0, kphase = 0, sphase = 1;
+            for (int j = 0; j < nb && ok; ++j) {
+                for (int t = 0; t < nt; ++t) {
+                    if (j + t > 0) ok = warp_wait(&bs->s_free, sphase, bs, p.status);  // the tile before has loaded its S
+                    sphase ^= 1;
+                    if (ok && t == 0) ok = warp_wait(&bs->k_full[ks], kphase, bs, p.status);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    if (tc::elect_one()) {
+                        const uint64_t qd = qd0 + (uint64_t)(t * (S::kQTile / 16)), kd = kd0 + (uint64_t)(ks * (S::kSlot / 16));
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
-                            tc::mma_bf16_ss(tmem + kColS, tc::sdesc_sw128(q_addr + (kk >> 2) * kHalf + (kk & 3) * 32, 16, 1024),
-                                            tc::sdesc_sw128(k_addr + (kk >> 2) * kHalf + (kk & 3) * 32, 16, 1024), idesc, kk > 0);
+                            tc::mma_bf16_ss(tmem + kColS, qd + (kk >> 2) * (kHalf / 16) + (kk & 3) * 2,
+                                            kd + (kk >> 2) * (kHalf / 16) + (kk & 3) * 2, idesc, kk > 0);
                         tc::mma_commit(&bs->s_full[t]);
-                        if (t == nt - 1) tc::mma_commit(&bs->k_empty[j % S::kKStages]);
+                        if (t == nt - 1) tc::mma_commit(&bs->k_empty[ks]);
                     }
+                    __syncwarp();
                 }
-                tc::mma_commit(&bs->drain);
-                tc::mbar_wait(&bs->drain, 0, kWaitBudget);
+                if (++ks == S::kKStages) {
+                    ks = 0;
+                    kphase ^= 1;
+                }
             }
+            if (tc::elect_one()) tc::mma_commit(&bs->drain);
+            __syncwarp();
+            tc::mbar_wait(&bs->drain, 0, kWaitBudget);
             __syncwarp();
         } else if (warp == kPvWarp) {
             // ---------------- PV issuer ----------------
             constexpr uint32_t idesc = tc::idesc_bf16_f32(128, D, true);
+            const uint64_t vd0 = tc::sdesc_sw128(tc::smem_u32(sm + S::kOffV), kHalf, 1024);
             bool ok = true;
+            int vs = 0, vphase = 0;
             for (int j = 0; j < nb && ok; ++j) {
-                const int vs = j % S::kVStages;
-                uint8_t *sV = sm + S::kOffV + vs * S::kSlot;
-                ok = __all_sync(0xffffffffu, wait_or_abort(&bs->v_full[vs], (j / S::kVStages) & 1, bs, p.status));
+                ok = warp_wait(&bs->v_full[vs], vphase, bs, p.status);
                 if (!ok) break;
                 // the page that holds the last visible position: zero its rows past it
                 const int end = kv_len - (blk0 + j) * kBlockKV;  // visible rows of the block
                 if (end < kBlockKV && (end & 15) != 0) {
+                    uint8_t *sV = sm + S::kOffV + vs * S::kSlot;
                     const int rows = 16 - (end & 15);
                     for (int i = lane; i < rows * 8 * S::kHalves; i += 32)
                         *reinterpret_cast<uint4 *>(sV + (i / (rows * 8)) * kHalf + end * 128 + (i % (rows * 8)) * 16) =
@@ -310,26 +322,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::fence_proxy_async_smem();
                     __syncwarp();
                 }
-                if (lane == 0) {
-                    const uint32_t v_addr = tc::smem_u32(sV);
-                    for (int t = 0; t < nt; ++t) {
-                        ok = wait_or_abort(&bs->p_full[t], j & 1, bs, p.status);
-                        if (!ok) break;
-                        tc::tc_fence_after();
+                for (int t = 0; t < nt; ++t) {
+                    ok = warp_wait(&bs->p_full[t], j & 1, bs, p.status);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    if (tc::elect_one()) {
+                        const uint64_t vd = vd0 + (uint64_t)(vs * (S::kSlot / 16));
 #pragma unroll
                         for (int kk = 0; kk < kBlockKV / 16; ++kk)
-                            tc::mma_bf16_ts(tmem + kColO + D * t, tmem + kColP + 64 * t + kk * 8,
-                                            tc::sdesc_sw128(v_addr + kk * 2048, kHalf, 1024), idesc, (j > 0 || kk > 0) ? 1u : 0u);
+                            tc::mma_bf16_ts(tmem + kColO + D * t, tmem + kColP + 64 * t + kk * 8, vd + kk * (2048 / 16), idesc,
+                                            (j > 0 || kk > 0) ? 1u : 0u);
                         tc::mma_commit(&bs->pv_done[t]);
                         if (t == nt - 1) tc::mma_commit(&bs->v_empty[vs]);
                     }
+                    __syncwarp();
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (++vs == S::kVStages) {
+                    vs = 0;
+                    vphase ^= 1;
+                }
             }
-            if (lane == 0) {
-                tc::mma_commit(&bs->drain_pv);
-                tc::mbar_wait(&bs->drain_pv, 0, kWaitBudget);
-            }
+            if (tc::elect_one()) tc::mma_commit(&bs->drain_pv);
+            __syncwarp();
+            tc::mbar_wait(&bs->drain_pv, 0, kWaitBudget);
             __syncwarp();
         }
     } else {
@@ -358,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int it = 0; it < nb && ok; ++it) {
                 const int p0 = (blk0 + it) * kBlockKV;
-                ok = __all_sync(0xffffffffu, wait_or_abort(&bs->s_full[tile], it & 1, bs, p.status));
+                ok = warp_wait(&bs->s_full[tile], it & 1, bs, p.status);
                 if (!ok) break;
                 tc::tc_fence_after();
                 float xa[64], xb[64];
@@ -403,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 // PV(it - 1) has read P and accumulated into O
                 if (it > 0) {
-                    ok = __all_sync(0xffffffffu, wait_or_abort(&bs->pv_done[tile], (it - 1) & 1, bs, p.status));
+                    ok = warp_wait(&bs->pv_done[tile], (it - 1) & 1, bs, p.status);
                     if (!ok) break;
                     tc::tc_fence_after();
                 }
@@ -441,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #undef X
             }
             // ---------------- epilogue ----------------
-            if (ok && __all_sync(0xffffffffu, wait_or_abort(&bs->pv_done[tile], (nb - 1) & 1, bs, p.status)) && warp_live) {
+            if (ok && warp_wait(&bs->pv_done[tile], (nb - 1) & 1, bs, p.status) && warp_live) {
                 tc::tc_fence_after();
                 // a row whose every score is -inf has no weight: zeros; a NaN stays one
                 const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;

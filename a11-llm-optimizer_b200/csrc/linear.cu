@@ -67,6 +67,11 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, Ba
     report(st, A11S_ETIMEOUT, (int32_t)blockIdx.x);
     return false;
 }
+// The same by a whole warp, with one answer for all its lanes (a converged warp stays one).
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, BarsCommon *bs, StatusWord *st) {
+    return __all_sync(0xffffffffu, wait_or_abort(bar, parity, bs, st));
+}
+__device__ __forceinline__ bool warp_aborted(BarsCommon *bs) { return __any_sync(0xffffffffu, aborted(bs)); }
 // The status word is cleared by the launch's first thread: a report can only
 // follow a wait of about a second, long after every CTA of the launch started.
 __device__ __forceinline__ void clear_status(StatusWord *st) {
@@ -129,18 +134,63 @@ __device__ __forceinline__ void write_rows(const float *stage, const LinParams &
     }
 }
 
-// This CTA's share (kOut / SPLIT columns) of the tile: the sums of the cluster's
-// CTAs, added in rank order, finished and written by the 128 epilogue threads t.
-// A thread takes four columns of every kPer-th group of rows, so that a warp's
-// loads from the other CTAs run along rows (whole lines: with a row per lane they
-// took 2400 cycles a step) and its columns' parameters stay in registers.
-template <bool GATED, int kOut, int SPLIT>
-__device__ __forceinline__ void merge_split(const float *part, const float *cols_sm, const float *xs_sm, const LinParams &p,
-                                            int rank, int t, int m0, int n0, bool params) {
+// What the 128 epilogue threads t of linear_tile do: under the wait for the
+// accumulator they fetch the residual; then the sums go to shared memory
+// (part, [128][BN + 4] fp32), and this CTA's share of the tile (kOut / SPLIT
+// columns) is added up over the cluster's CTAs in rank order, finished and
+// written. There a thread takes four columns of every kPer-th group of rows, so
+// that a warp's loads from the other CTAs run along rows (whole lines: with a row
+// per lane they took 2400 cycles a step of 8 columns) and its columns' parameters
+// stay in registers. Reading another CTA's sums runs at some 10 bytes per cycle:
+// splits that leave a CTA few columns are the cheap ones.
+template <bool GATED, int BN, int SPLIT>
+__device__ __forceinline__ void tile_epilogue(TileBars *bs, float *part, const float *cols_sm, const float *xs_sm, const LinParams &p,
+                                              uint32_t tmem, int ns, int rank, int t, int m0, int n0, bool params) {
+    constexpr int kOut = GATED ? BN / 2 : BN;
     constexpr int kCols = kOut / SPLIT, kPer = kCols / 4, kStep = kTileM / kPer;  // threads of a row, rows of a pass
-    constexpr int kPitch = (GATED ? 2 * kOut : kOut) + 4;
+    constexpr int kPitch = BN + 4;
     constexpr int kBatch = kPer < 2 ? 1 : SPLIT * (GATED ? 2 : 1) <= 8 && kPer >= 4 ? 4 : 2;  // passes in flight
     const int c = rank * kCols + t % kPer * 4, r0 = t / kPer, n = n0 + c;
+    uint2 res[kBatch];  // four bf16 of each pass of the next batch; absent elements: the last ones again
+    auto load_residual = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            res[i] = make_uint2(0, 0);
+            if (!p.residual) continue;
+            const __nv_bfloat16 *row = p.residual + (int64_t)min(m0 + r0 + (i0 + i) * kStep, p.rows - 1) * p.res_stride;
+            if (p.vec4) {
+                res[i] = *reinterpret_cast<const uint2 *>(row + min(n, p.N - 4));
+            } else {
+                const uint16_t *e = reinterpret_cast<const uint16_t *>(row);
+                res[i].x = e[min(n, p.N - 1)] | (uint32_t)e[min(n + 1, p.N - 1)] << 16;
+                res[i].y = e[min(n + 2, p.N - 1)] | (uint32_t)e[min(n + 3, p.N - 1)] << 16;
+            }
+        }
+    };
+    load_residual(0);
+    const bool ok = warp_wait(&bs->acc_full, 0, bs, p.status);
+    tc::tc_fence_after();
+    const int row = ((threadIdx.x >> 5) & 3) * 32 + (t & 31);  // TMEM lane = tile row: warp % 4 chooses the lanes
+    if (ok) {
+#pragma unroll
+        for (int e0 = 0; e0 < BN; e0 += 32) {
+            float v[32];
+            if (ns > 0) {
+                tc::tmem_ld32(tmem + ((uint32_t)(row & 96) << 16) + e0, v);
+            } else {  // no K slice fell to this CTA
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4 *>(part + row * kPitch + e0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        }
+    }
+    __syncwarp();
+    // every CTA's sums are in shared memory (after a timeout nobody waits for them)
+    if (SPLIT == 1) epilogue_barrier<128>();
+    else tc::cluster_sync();
+    if (!ok) return;
     float4 ws = make_float4(1, 1, 1, 1), wb = make_float4(0, 0, 0, 0), gs = ws, gb = wb;
     if (params) {
         ws = *reinterpret_cast<const float4 *>(cols_sm + c);
@@ -153,33 +203,26 @@ __device__ __forceinline__ void merge_split(const float *part, const float *cols
     uint32_t src[SPLIT];
 #pragma unroll
     for (int r = 0; r < SPLIT; ++r) src[r] = tc::cluster_addr(part, r) + (uint32_t)(r0 * kPitch + c) * 4;
+    // rolled: code that runs once costs its fetching (unrolled, 32 passes took 6 us longer)
 #pragma unroll 1
     for (int i0 = 0; i0 < kPer; i0 += kBatch) {
-        float4 a[kBatch][SPLIT], g[GATED ? kBatch : 1][GATED ? SPLIT : 1], res[kBatch];
+        uint2 add[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < kBatch; ++i) add[i] = res[i];
+        if (i0 + kBatch < kPer) load_residual(i0 + kBatch);  // rows that this batch does not write
+        float4 a[kBatch][SPLIT], g[GATED ? kBatch : 1][GATED ? SPLIT : 1];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
 #pragma unroll
             for (int r = 0; r < SPLIT; ++r) {
                 const uint32_t at = src[r] + (uint32_t)((i0 + i) * kStep * kPitch) * 4;
                 a[i][r] = tc::ld_cluster_v4(at + (GATED ? kOut * 4 : 0));
                 if constexpr (GATED) g[i][r] = tc::ld_cluster_v4(at);
             }
-            res[i] = make_float4(0, 0, 0, 0);
-            if (p.residual) {  // absent elements: the last ones again
-                const __nv_bfloat16 *row = p.residual + (int64_t)min(m0 + r0 + (i0 + i) * kStep, p.rows - 1) * p.res_stride;
-                if (p.vec4) {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(row + min(n, p.N - 4));
-                    res[i] = make_float4(bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y));
-                } else {
-                    res[i] = make_float4(__bfloat162float(row[min(n, p.N - 1)]), __bfloat162float(row[min(n + 1, p.N - 1)]),
-                                         __bfloat162float(row[min(n + 2, p.N - 1)]), __bfloat162float(row[min(n + 3, p.N - 1)]));
-                }
-            }
-        }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int row = r0 + (i0 + i) * kStep, m = m0 + row;
-            const float xs = params ? xs_sm[row] : 1.0f;
+            const int rr = r0 + (i0 + i) * kStep, m = m0 + rr;
+            const float xs = params ? xs_sm[rr] : 1.0f;
             float4 v = a[i][0], u = make_float4(0, 0, 0, 0);
             if constexpr (GATED) u = g[i][0];
 #pragma unroll
@@ -187,10 +230,11 @@ __device__ __forceinline__ void merge_split(const float *part, const float *cols
                 v = make_float4(v.x + a[i][r].x, v.y + a[i][r].y, v.z + a[i][r].z, v.w + a[i][r].w);
                 if constexpr (GATED) u = make_float4(u.x + g[i][r].x, u.y + g[i][r].y, u.z + g[i][r].z, u.w + g[i][r].w);
             }
-            const float y0 = finish<GATED>(v.x, u.x, xs, Column{ws.x, wb.x, gs.x, gb.x}, p.act) + res[i].x;
-            const float y1 = finish<GATED>(v.y, u.y, xs, Column{ws.y, wb.y, gs.y, gb.y}, p.act) + res[i].y;
-            const float y2 = finish<GATED>(v.z, u.z, xs, Column{ws.z, wb.z, gs.z, gb.z}, p.act) + res[i].z;
-            const float y3 = finish<GATED>(v.w, u.w, xs, Column{ws.w, wb.w, gs.w, gb.w}, p.act) + res[i].w;
+            const uint2 w = add[i];
+            const float y0 = finish<GATED>(v.x, u.x, xs, Column{ws.x, wb.x, gs.x, gb.x}, p.act) + bf16lo(w.x);
+            const float y1 = finish<GATED>(v.y, u.y, xs, Column{ws.y, wb.y, gs.y, gb.y}, p.act) + bf16hi(w.x);
+            const float y2 = finish<GATED>(v.z, u.z, xs, Column{ws.z, wb.z, gs.z, gb.z}, p.act) + bf16lo(w.y);
+            const float y3 = finish<GATED>(v.w, u.w, xs, Column{ws.w, wb.w, gs.w, gb.w}, p.act) + bf16hi(w.y);
             if (m < p.rows) {
                 __nv_bfloat16 *o = p.out + (int64_t)m * p.out_stride + n;
                 if (p.vec4) {
@@ -217,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     TileBars *bs = reinterpret_cast<TileBars *>(sm + S::kOffBars);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
     const int rank = blockIdx.x % p.split, tile = blockIdx.x / p.split;  // clusters are consecutive CTAs
     const int m0 = (tile % p.m_tiles) * kTileM, n0 = (tile / p.m_tiles) * kOut;
     const int per = (p.slices + p.split - 1) / p.split;
@@ -243,15 +287,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = bs->tmem_base;
 
     if (warp == 0) {
-        if (lane == 0) {
-            constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
+        constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
+        if (tc::elect_one()) {
             tc::prefetch_tmap(&tx);
             tc::prefetch_tmap(&tw);
             if (GATED) tc::prefetch_tmap(&tg);
-            for (int i = 0; i < ns; ++i) {
-                const int s = i % S::kStages, use = i / S::kStages;
-                if (use > 0 && !wait_or_abort(&bs->empty[s], (use - 1) & 1, bs, p.status)) break;
-                if (aborted(bs)) break;
+        }
+        for (int i = 0, s = 0, use = 0; i < ns; ++i) {
+            if (use > 0 && !warp_wait(&bs->empty[s], (use - 1) & 1, bs, p.status)) break;
+            if (warp_aborted(bs)) break;
+            if (tc::elect_one()) {
                 uint8_t *a = sm + s * S::kStage;
                 const int k = (s0 + i) * kElems;
                 tc::mbar_arrive_expect_tx(&bs->full[s], S::kStage);
@@ -263,102 +308,62 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::tma_load_2d(a + kTileABytes, &tw, &bs->full[s], k, n0);
                 }
             }
+            __syncwarp();
+            if (++s == S::kStages) {
+                s = 0;
+                ++use;
+            }
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = E4M3 ? tc::idesc_e4m3_f32(kTileM, BN) : tc::idesc_bf16_f32(kTileM, BN, false);
-            bool ok = true;
-            for (int i = 0; i < ns && ok; ++i) {
-                const int s = i % S::kStages;
-                if (!(ok = wait_or_abort(&bs->full[s], (i / S::kStages) & 1, bs, p.status))) break;
-                tc::tc_fence_after();
-                const uint32_t a = tc::smem_u32(sm + s * S::kStage), b = a + kTileABytes;
+        constexpr uint32_t idesc = E4M3 ? tc::idesc_e4m3_f32(kTileM, BN) : tc::idesc_bf16_f32(kTileM, BN, false);
+        const uint64_t ad0 = tc::sdesc_sw128(tc::smem_u32(sm), 16, 1024);  // + 16-byte units: slots, 32 bytes per MMA
+        bool ok = true;
+        for (int i = 0, s = 0, use = 0; i < ns; ++i) {
+            if (!(ok = warp_wait(&bs->full[s], use & 1, bs, p.status))) break;
+            tc::tc_fence_after();
+            if (tc::elect_one()) {
+                const uint64_t ad = ad0 + (uint64_t)(s * (S::kStage / 16)), bd = ad + kTileABytes / 16;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
-                    const uint64_t ad = tc::sdesc_sw128(a + kk * 32, 16, 1024), bd = tc::sdesc_sw128(b + kk * 32, 16, 1024);
-                    if constexpr (E4M3) tc::mma_e4m3_ss(tmem, ad, bd, idesc, (i | kk) != 0);
-                    else tc::mma_bf16_ss(tmem, ad, bd, idesc, (i | kk) != 0);
+                    if constexpr (E4M3) tc::mma_e4m3_ss(tmem, ad + 2 * kk, bd + 2 * kk, idesc, (i | kk) != 0);
+                    else tc::mma_bf16_ss(tmem, ad + 2 * kk, bd + 2 * kk, idesc, (i | kk) != 0);
                 }
                 tc::mma_commit(&bs->empty[s]);
             }
+            __syncwarp();
+            if (++s == S::kStages) {
+                s = 0;
+                ++use;
+            }
+        }
+        if (tc::elect_one()) {
             if (ok) tc::mma_commit(&bs->acc_full);
             tc::mma_commit(&bs->drain);
-            tc::mbar_wait(&bs->drain, 0, kWaitBudget);
         }
         __syncwarp();
+        tc::mbar_wait(&bs->drain, 0, kWaitBudget);
+        __syncwarp();
     }
-    // ---------------- epilogue warps ----------------
-    const int q = warp & 3, row = q * 32 + lane, m = m0 + row;  // TMEM lane = tile row
-    const uint32_t lane_base = (uint32_t)(q * 32) << 16;
-    float *cols_sm = reinterpret_cast<float *>(sm + S::kOffCols), *xs_sm = cols_sm + 512;
-    const bool params = p.col.any();
-    float xs = 1.0f;
-    bool ok = true;
     if (warp >= 2) {
-        if (params) stage_columns<GATED, kOut>(cols_sm, p.col, n0, p.N, threadIdx.x - 64, 128);
-        if (E4M3 && m < p.rows) xs = __ldg(p.x_scale + m);
-        if (params) xs_sm[row] = xs;
+        const int t = threadIdx.x - 64;
+        float *cols_sm = reinterpret_cast<float *>(sm + S::kOffCols), *xs_sm = cols_sm + 512, *part = reinterpret_cast<float *>(sm);
+        const bool params = p.col.any();
+        if (params) {
+            stage_columns<GATED, kOut>(cols_sm, p.col, n0, p.N, t, 128);
+            xs_sm[t] = E4M3 && m0 + t < p.rows ? __ldg(p.x_scale + m0 + t) : 1.0f;
+        }
         epilogue_barrier<128>();
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bs->acc_full, 0, bs, p.status));
-        tc::tc_fence_after();
-    }
-    // With the accumulator complete the ring is free. part: this CTA's sums,
-    // [128][BN + 4] fp32; stage: finished outputs of an epilogue warp.
-    float *part = reinterpret_cast<float *>(sm);
-    float *stage = part + kTileM * (BN + 4) + q * 32 * (kOut + 1);
-    if (p.split == 1) {
-        constexpr int kW = kOut < 32 ? kOut : 32;
-        if (warp >= 2 && ok) {
-#pragma unroll 1
-            for (int c = 0; c < kOut; c += kW) {
-                float v[kW], u[GATED ? kW : 1];
-                if constexpr (kW == 32) {
-                    tc::tmem_ld32(tmem + lane_base + (GATED ? kOut : 0) + c, v);
-                    if constexpr (GATED) tc::tmem_ld32(tmem + lane_base + c, u);
-                } else {  // gate and weight columns side by side
-                    float both[32];
-                    tc::tmem_ld32(tmem + lane_base, both);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        u[e] = both[e];
-                        v[e] = both[16 + e];
-                    }
-                }
-                finish_columns<GATED, kOut>(v, u, xs, cols_sm, c, params, p.act);
-#pragma unroll
-                for (int e = 0; e < kW; ++e) stage[lane * (kW + 1) + e] = v[e];
-                __syncwarp();
-                write_rows<kW>(stage, p, m0 + q * 32, n0 + c, lane);
-                __syncwarp();
-            }
-        }
-    } else {
-        if (warp >= 2 && ok) {
-#pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                float v[32];
-                if (ns > 0) {
-                    tc::tmem_ld32(tmem + lane_base + c, v);
-                } else {  // no K slice fell to this CTA
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = 0.0f;
-                }
-#pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    *reinterpret_cast<float4 *>(part + row * (BN + 4) + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-            }
-        }
+        auto run = [&](auto split) {
+            tile_epilogue<GATED, BN, decltype(split)::value>(bs, part, cols_sm, xs_sm, p, tmem, ns, rank, t, m0, n0, params);
+        };
+        if (p.split == 1) run(std::integral_constant<int, 1>{});
+        else if (p.split == 2) run(std::integral_constant<int, 2>{});
+        else if (p.split == 4) run(std::integral_constant<int, 4>{});
+        else if constexpr (kOut >= 32) run(std::integral_constant<int, 8>{});
+    } else if (p.split > 1) {
         __syncwarp();
-        tc::cluster_sync();  // every CTA's sums are in shared memory (and after a timeout nobody waits for them)
-        if (warp >= 2 && ok) {
-            auto merge = [&](auto split) {
-                merge_split<GATED, kOut, decltype(split)::value>(part, cols_sm, xs_sm, p, rank, threadIdx.x - 64, m0, n0, params);
-            };
-            if (p.split == 2) merge(std::integral_constant<int, 2>{});
-            else if (p.split == 4) merge(std::integral_constant<int, 4>{});
-            else if constexpr (kOut >= 32) merge(std::integral_constant<int, 8>{});
-        }
+        tc::cluster_sync();  // the epilogue warps' one
     }
     // After a timeout copies may still be landing here: give them time (about
     // 0.2 ms) before the shared memory is released.
@@ -439,60 +444,70 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t tmem = bs->tmem_base;
 
     if (warp == 0) {
-        if (lane == 0) {
-            constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
-            // B rows of this CTA: gated, the even CTA stages the gate's rows and the odd one the weight's
-            const CUtensorMap *tb = GATED && rank == 0 ? &tg : &tw;
-            int it = 0;
-            bool ok = true;
-            for (int i = 0; i < my_tiles && ok; ++i) {
-                const int t = unit + i * units;
-                const int m0 = (t % p.m_tiles) * kPairM + (int)rank * 128;
-                const int nb = (t / p.m_tiles) * kOut + (GATED ? 0 : (int)rank * 128);
-                for (int kb = 0; kb < p.slices; ++kb) {
-                    const int s = it % kPairStages, use = it / kPairStages;
-                    if (use > 0 && !(ok = wait_or_abort(&bs->empty[s], (use - 1) & 1, bs, p.status))) break;
-                    if (aborted(bs)) {
-                        ok = false;
-                        break;
-                    }
+        constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
+        // B rows of this CTA: gated, the even CTA stages the gate's rows and the odd one the weight's
+        const CUtensorMap *tb = GATED && rank == 0 ? &tg : &tw;
+        int s = 0, use = 0;
+        bool ok = true;
+        for (int i = 0; i < my_tiles && ok; ++i) {
+            const int t = unit + i * units;
+            const int m0 = (t % p.m_tiles) * kPairM + (int)rank * 128;
+            const int nb = (t / p.m_tiles) * kOut + (GATED ? 0 : (int)rank * 128);
+            for (int kb = 0; kb < p.slices; ++kb) {
+                if (use > 0 && !(ok = warp_wait(&bs->empty[s], (use - 1) & 1, bs, p.status))) break;
+                if (warp_aborted(bs)) {
+                    ok = false;
+                    break;
+                }
+                if (tc::elect_one()) {
                     uint8_t *a = sm + s * kPairStage;
                     const uint32_t fb = tc::cluster_addr(&bs->full[s], 0);
                     if (rank == 0) tc::mbar_arrive_expect_tx(&bs->full[s], 2 * kPairStage);
                     tc::tma_load_2d_pair(a, &tx, fb, kb * kElems, m0);
                     tc::tma_load_2d_pair(a + kPairHalf, tb, fb, kb * kElems, nb);
-                    ++it;
+                }
+                __syncwarp();
+                if (++s == kPairStages) {
+                    s = 0;
+                    ++use;
                 }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             constexpr uint32_t idesc = E4M3 ? tc::idesc_e4m3_f32(kPairM, kPairN) : tc::idesc_bf16_f32(kPairM, kPairN, false);
-            int it = 0;
+            const uint64_t ad0 = tc::sdesc_sw128(tc::smem_u32(sm), 16, 1024);
+            int s = 0, phase = 0;
             bool ok = true;
             for (int i = 0; i < my_tiles && ok; ++i) {
                 const int buf = i & 1, use = i >> 1;
-                if (use > 0 && !(ok = wait_or_abort(&bs->acc_empty[buf], (use - 1) & 1, bs, p.status))) break;
+                if (use > 0 && !(ok = warp_wait(&bs->acc_empty[buf], (use - 1) & 1, bs, p.status))) break;
                 tc::tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)(buf * kPairN);
                 for (int kb = 0; kb < p.slices; ++kb) {
-                    const int s = it % kPairStages;
-                    if (!(ok = wait_or_abort(&bs->full[s], (it / kPairStages) & 1, bs, p.status))) break;
+                    if (!(ok = warp_wait(&bs->full[s], phase, bs, p.status))) break;
                     tc::tc_fence_after();
-                    const uint32_t a = tc::smem_u32(sm + s * kPairStage), b = a + kPairHalf;
+                    if (tc::elect_one()) {
+                        const uint64_t ad = ad0 + (uint64_t)(s * (kPairStage / 16)), bd = ad + kPairHalf / 16;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t ad = tc::sdesc_sw128(a + kk * 32, 16, 1024), bd = tc::sdesc_sw128(b + kk * 32, 16, 1024);
-                        if constexpr (E4M3) tc::mma_e4m3_ss_pair(d, ad, bd, idesc, (kb | kk) != 0);
-                        else tc::mma_bf16_ss_pair(d, ad, bd, idesc, (kb | kk) != 0);
+                        for (int kk = 0; kk < 4; ++kk) {
+                            if constexpr (E4M3) tc::mma_e4m3_ss_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, (kb | kk) != 0);
+                            else tc::mma_bf16_ss_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, (kb | kk) != 0);
+                        }
+                        tc::mma_commit_pair_both(&bs->empty[s]);
                     }
-                    tc::mma_commit_pair_both(&bs->empty[s]);
-                    ++it;
+                    __syncwarp();
+                    if (++s == kPairStages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
-                if (ok) tc::mma_commit_pair_both(&bs->acc_full[buf]);
+                if (ok && tc::elect_one()) tc::mma_commit_pair_both(&bs->acc_full[buf]);
+                __syncwarp();
             }
-            tc::mma_commit_pair(&bs->drain);
+            if (tc::elect_one()) tc::mma_commit_pair(&bs->drain);
+            __syncwarp();
             tc::mbar_wait(&bs->drain, 0, kWaitBudget);
         }
         __syncwarp();
@@ -527,7 +542,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 for (int c = 0; c < 4; ++c) res[c] = in && n + 8 * c < p.N ? __ldcs(src + c) : make_uint4(0, 0, 0, 0);
             };
             if (p.vec_res) load_residual(n0 + first * kEpiCols);
-            ok = __all_sync(0xffffffffu, wait_or_abort(&bs->acc_full[buf], (i >> 1) & 1, bs, p.status));
+            ok = warp_wait(&bs->acc_full[buf], (i >> 1) & 1, bs, p.status);
             if (!ok) break;
             tc::tc_fence_after();
 #pragma unroll 1
@@ -643,31 +658,55 @@ int device_sms() {
     return v;
 }
 
-// What a tiling costs, in cycles: waves of tiles, each its K slices and what a
-// tile spends besides (filling the ring, the epilogue).
+// Clusters of `split` linear_tile CTAs that can be resident at once.
+int tile_slots(int split, int sms) {
+    static std::atomic<int> known[4] = {};  // splits 1, 2, 4, 8; every instantiation fills an SM with one CTA
+    const int i = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
+    int v = known[i].load();
+    if (!v) {
+        auto kernel = linear_tile<false, false, 64>;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(sms / split * split));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = TileShape<64>::kSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)split;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<64>::kSmem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) != cudaSuccess || v < 1)
+            v = std::max(1, sms / split * (split == 8 ? 3 : 4) / 4);
+        known[i].store(v);
+    }
+    return v;
+}
+
+// What a tiling takes, in microseconds: waves of tiles, each its K slices and
+// what a tile spends besides (filling the ring, exchanging sums, the epilogue).
+// Fitted to a sweep of every (BN, split) over 14 sizes of 48 to 2048 rows, K 512
+// to 8192 and N 200 to 8192; the choice was the fastest there or within 6 % of it.
+// For instance 64 x 8192 -> 2048: 64/4 14.2 us, 32/2 18.7, 64/1 33.6, pairs 43.9;
+// 768 x 4096 -> 4096: pairs 26.3, 128/2 45.5; 197 x 1000 -> 1531: 64/2 10.0, 32/1 10.4.
 struct Plan {
     int bn = 0, split = 1;  // bn 0: linear_pair
-    double cost = 1e300;
 };
 Plan choose(const LinearArgs &a, int slices, int sms) {
+    const auto tiles = [&](int m, int n) { return (long long)((a.rows + m - 1) / m) * ((a.N + n - 1) / n); };
     Plan best;
-    const auto tiles = [&](int m, int n) {
-        return (long long)((a.rows + m - 1) / m) * ((a.N + n - 1) / n);
-    };
-    {
-        const long long t = tiles(kPairM, a.gate ? kPairN / 2 : kPairN);
-        const double waves = (double)((t + sms / 2 - 1) / (sms / 2));
-        best.cost = waves * (slices * 540.0) + 5000.0;
-    }
+    const long long pairs = tiles(kPairM, a.gate ? kPairN / 2 : kPairN);
+    double least = (double)((pairs + sms / 2 - 1) / (sms / 2)) * slices * 0.32 + 6.0;
     for (int bn : {32, 64, 128})
         for (int split : {1, 2, 4, 8}) {
             if (split > 1 && (split > slices || (bn == 32 && a.gate && split == 8))) break;
-            const long long t = tiles(kTileM, a.gate ? bn / 2 : bn) * split;
-            const double waves = (double)((t + sms - 1) / sms);
-            const double per = (slices + split - 1) / split;
-            const double cost = waves * (per * (bn == 32 ? 340.0 : bn == 64 ? 400.0 : 540.0) + 3500.0 + (split > 1 ? 1500.0 : 0.0));
-            if (cost < best.cost) {
-                best.cost = cost;
+            const double slice = bn == 32 ? 0.20 : bn == 64 ? 0.21 : 0.235;
+            const double fixed = split == 1 ? 3.05 + 0.045 * bn : split == 2 ? 3.55 + 0.0266 * bn : split == 4 ? 4.1 + 0.018 * bn
+                                                                                                       : 4.9 + 0.03 * bn;
+            const long long t = tiles(kTileM, a.gate ? bn / 2 : bn), slots = tile_slots(split, sms);
+            const double us = (double)((t + slots - 1) / slots) * ((slices + split - 1) / split * slice + fixed);
+            if (us < least) {
+                least = us;
                 best.bn = bn;
                 best.split = split;
             }
