@@ -664,7 +664,7 @@ int a11s_chunk_attention(const void *q, int64_t q_stride, const void *k_pool, co
     a.part_o = reinterpret_cast<float *>(ws + lay.part_o);
     a.part_ml = reinterpret_cast<float *>(ws + lay.part_ml);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = cudaMemsetAsync(ws, 0, a.plan.rows ? lay.part_o : sizeof(a11s::StatusWord), s);
+    cudaError_t e = a11s::launch_chunk_attention_clear(ws, a.plan.rows ? lay.part_o : sizeof(a11s::StatusWord), s);
     if (e != cudaSuccess) return cuda_fail(e, "a11s_chunk_attention: clearing status");
     e = a11s::launch_chunk_attention(a, s);
     if (e != cudaSuccess) return cuda_fail(e, "a11s_chunk_attention: launch");

@@ -137,6 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Bars *bs = reinterpret_cast<Bars *>(sm + S::kOffBar);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    let_next_start();
+    wait_before();
     // the chunk's last tokens see the most keys: they start first
     int idx = blockIdx.x;
     const int g = idx % p.Hkv;
@@ -513,6 +515,8 @@ __global__ void __launch_bounds__(D) chunk_attn_combine(const Params p) {
     __shared__ float weight[kMaxSplits];
     __shared__ float total[2];
     const size_t row = blockIdx.x, rows = (size_t)p.B * p.N * p.Hq;
+    let_next_start();
+    wait_before();
     const int t = threadIdx.x, b = (int)(row / ((size_t)p.N * p.Hq)), token = (int)((row / p.Hq) % p.N);
     int L;
     const int n_live = live_tokens(p, b, L, false);
@@ -559,6 +563,19 @@ __global__ void __launch_bounds__(D) chunk_attn_combine(const Params p) {
 }
 
 // ---------------------------------------------------------------------------- host side
+// Clears the status word and the merge counters: a kernel and not a memset, so
+// that the attention can start over its tail.
+namespace {
+__global__ void chunk_attn_clear(uint32_t *words, int n) {
+    let_next_start();
+    wait_before();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) words[i] = 0;
+}
+}  // namespace
+cudaError_t launch_chunk_attention_clear(void *workspace, size_t bytes, cudaStream_t s) {
+    return launch_overlapped(chunk_attn_clear, dim3(1), 256, 0, 1, s, static_cast<uint32_t *>(workspace), (int)(bytes / 4));
+}
+
 ChunkPlan chunk_attention_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t max_kv_len) {
     const int max_pages = (max_kv_len + A11S_PAGE_TOKENS - 1) / A11S_PAGE_TOKENS;
     int sms = 148, dev = 0;
@@ -631,11 +648,10 @@ cudaError_t launch_d(const ChunkAttnArgs &a, const Params &p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     // setmaxnreg.inc would wait forever if the split needed more registers than the launch holds
     if ((long long)fa.numRegs * kThreads < kRegsNeeded) return cudaErrorInvalidConfiguration;
-    kernel<<<(unsigned)((long long)p.ctiles * p.B * p.splits * p.Hkv), kThreads, Shape<D>::kSmem, s>>>(tk, tv, p);
-    e = cudaGetLastError();
+    e = launch_overlapped(kernel, dim3((unsigned)((long long)p.ctiles * p.B * p.splits * p.Hkv)), kThreads, Shape<D>::kSmem, 1, s,
+                          tk, tv, p);
     if (e != cudaSuccess || p.splits == 1) return e;
-    chunk_attn_combine<D><<<(unsigned)((size_t)p.B * p.N * p.Hq), D, 0, s>>>(p);
-    return cudaGetLastError();
+    return launch_overlapped(chunk_attn_combine<D>, dim3((unsigned)((size_t)p.B * p.N * p.Hq)), D, 0, 1, s, p);
 }
 }  // namespace
 

@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_rows(const Params p) {
     __shared__ int is_last, warp_sum[kWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
 
+    let_next_start();
+    wait_before();
     // ---------------- pages of the sequences, summed up ----------------
     {
         const int per = (p.B + kThreads - 1) / kThreads, b0 = tid * per;
@@ -121,19 +123,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_rows(const Params p) {
         }
     }
     // this CTA's share: pages [r0, r1) of all, or (short sequences) whole units.
-    // All counts fit 32 bits (checked on the host); shares * shares does too.
+    // All counts fit 32 bits (checked on the host).
     const int units = p.B * p.Hkv, total = prefix[p.B] * p.Hkv;
     if (total == 0) return;
     const bool whole = total <= units * 16ll;
     const int shares = min((int)gridDim.x, whole ? units : (total + kMinPages - 1) / kMinPages), me = blockIdx.x;
     if (me >= shares) return;
-    const int each = total / shares, extra = total % shares;
-    auto share_start = [&](int c) { return each * c + extra * c / shares; };  // total * c / shares
+    const int each = total / shares, extra = total % shares;  // the first `extra` shares have a page more
+    auto share_start = [&](int c) { return each * c + min(c, extra); };
     auto share_of = [&](int x) {  // the CTA whose share holds page x
-        int c = min(shares - 1, (int)((float)x * ((float)shares / (float)total)));
-        while (share_start(c) > x) --c;
-        while (c + 1 < shares && share_start(c + 1) <= x) ++c;
-        return c;
+        const int longer = extra * (each + 1);
+        return x < longer ? x / (each + 1) : extra + (x - longer) / each;
     };
     const int r0 = whole ? 0 : share_start(me), r1 = whole ? 0 : share_start(me + 1);
     // the first unit: (b, g), and the page it starts at
@@ -384,20 +384,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_rows(const Params p) {
                     // pieces' outputs, copied there all at once (as many as fit) while the weights
                     // are formed. Every thread copies and later reads elements of its own.
                     float *wgt = reinterpret_cast<float *>(smem);
-                    constexpr uint32_t kStageAt = kChunkRows * kMaxShares * 4;
-                    constexpr int kSlots = (kWarps * S::kRing - kStageAt) / (kThreads * 16);
-                    constexpr int kRowThreads = kThreads / kDims4;         // rows side by side
-                    const int nr = (rows + kRowThreads - 1) / kRowThreads;  // rows of a thread
-                    const int group = kSlots / nr;                          // pieces at a time
+                    constexpr uint32_t kStageAt = kRows * kMaxShares * 4;
+                    constexpr int kRowThreads = kThreads / kDims4;                    // rows side by side
+                    constexpr int kNr = (kRows + kRowThreads - 1) / kRowThreads;      // rows of a thread
+                    constexpr int kGroup = (kWarps * S::kRing - kStageAt) / (kThreads * 16) / kNr;  // pieces at a time
+                    auto my_row = [&](int k) { return min(tid / kDims4 + k * kRowThreads, kRows - 1); };
                     const uint32_t mine16 = tc::smem_u32(smem) + kStageAt + tid * 16;
-                    auto slot_of = [&](int i) { return 2 * (size_t)(c0 + i) + (i == 0 ? 1 : 0); };
+                    // piece i of the unit sits in slot 2 (c0 + i), the first one in 2 c0 + 1
+                    const float *piece0 = p.part_o + (size_t)2 * c0 * kRows * D + d4;
+                    const float *ml0 = p.part_ml + (size_t)2 * c0 * kRows * 2;
                     auto fetch = [&](int i0) {
-                        for (int i = 0; i < group && i0 + i < n; ++i) {
-                            const float *src = p.part_o + slot_of(i0 + i) * kRows * D + d4;
-                            for (int k = 0; k < nr; ++k) {
-                                const int r = tid / kDims4 + k * kRowThreads;
-                                cp_async16(mine16 + (i * nr + k) * (kThreads * 16), src + (r < rows ? r : 0) * D, true);
-                            }
+                        const int m = min(kGroup, n - i0);
+#pragma unroll 4
+                        for (int i = 0; i < m; ++i) {
+                            const float *src = piece0 + (2 * (i0 + i) + (i0 + i == 0)) * (kRows * D);
+#pragma unroll
+                            for (int k = 0; k < kNr; ++k)  // rows past the last hold nothing and are not used
+                                cp_async16(mine16 + (i * kNr + k) * (kThreads * 16), src + my_row(k) * D, true);
                         }
                         cp_async_commit();
                     };
@@ -406,10 +409,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_rows(const Params p) {
                         float2 v[kMaxShares / 32];
                         float M = -INFINITY, sum = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < kMaxShares / 32; ++i)
-                            v[i] = lane + 32 * i < n
-                                       ? __ldcg(reinterpret_cast<const float2 *>(p.part_ml + (slot_of(lane + 32 * i) * kRows + r) * 2))
-                                       : make_float2(-INFINITY, 0.0f);
+                        for (int i = 0; i < kMaxShares / 32; ++i) {
+                            const int at = lane + 32 * i;
+                            v[i] = make_float2(-INFINITY, 0.0f);
+                            if (at < n) v[i] = __ldcg(reinterpret_cast<const float2 *>(ml0 + ((2 * at + (at == 0)) * kRows + r) * 2));
+                        }
 #pragma unroll
                         for (int i = 0; i < kMaxShares / 32; ++i) M = fmaxf(M, v[i].x);
                         M = warp_fmax(M);
@@ -423,24 +427,26 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_rows(const Params p) {
                         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-                        for (int i = 0; i < kMaxShares / 32; ++i)
+                        for (int i = 0; i < kMaxShares / 32; ++i) {
+                            if (32 * i >= n) break;
                             if (lane + 32 * i < n) wgt[r * kMaxShares + lane + 32 * i] = v[i].x * inv;
+                        }
                         if (p.lse && lane == 0) p.lse[row_of(r)] = sum == 0.0f ? 0.0f : (M + log2f(sum)) * 0.6931471805599453f;
                     }
                     __syncthreads();
-                    float4 acc[4];  // nr <= 4: at most 32 rows, at least 8 side by side
+                    float4 acc[kNr];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0, 0, 0, 0);
-                    for (int i0 = 0; i0 < n; i0 += group) {
+                    for (int k = 0; k < kNr; ++k) acc[k] = make_float4(0, 0, 0, 0);
+                    for (int i0 = 0; i0 < n; i0 += kGroup) {
                         if (i0 > 0) fetch(i0);
                         cp_async_wait<0>();
-                        for (int i = 0; i < group && i0 + i < n; ++i)
+                        const int m = min(kGroup, n - i0);
+#pragma unroll 8
+                        for (int i = 0; i < m; ++i)
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const int r = tid / kDims4 + k * kRowThreads;
-                                if (r >= rows) break;
-                                const float f = wgt[r * kMaxShares + i0 + i];
-                                const float4 a = *reinterpret_cast<const float4 *>(smem + kStageAt + tid * 16 + (i * nr + k) * (kThreads * 16));
+                            for (int k = 0; k < kNr; ++k) {
+                                const float f = wgt[my_row(k) * kMaxShares + i0 + i];
+                                const float4 a = *reinterpret_cast<const float4 *>(smem + kStageAt + tid * 16 + (i * kNr + k) * (kThreads * 16));
                                 const bool seen = f != 0.0f;  // else whatever is there takes no part
                                 acc[k].x = fmaf(f, seen ? a.x : 0.0f, acc[k].x);
                                 acc[k].y = fmaf(f, seen ? a.y : 0.0f, acc[k].y);
@@ -449,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_rows(const Params p) {
                             }
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                    for (int k = 0; k < kNr; ++k) {
                         const int r = tid / kDims4 + k * kRowThreads;
                         if (r < rows)
                             *reinterpret_cast<uint2 *>(p.out + row_of(r) * D + d4) =
@@ -485,8 +491,7 @@ cudaError_t launch_rows_d(const Params &p, int ctas, cudaStream_t s) {
     auto go = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
         if (e != cudaSuccess) return e;
-        kernel<<<ctas, kThreads, Shape<D>::kSmem, s>>>(p);
-        return cudaGetLastError();
+        return launch_overlapped(kernel, dim3(ctas), kThreads, Shape<D>::kSmem, 1, s, p);
     };
     switch ((p.N * p.group + 7) / 8) {
         case 1: return go(chunk_attn_rows<D, 1>);

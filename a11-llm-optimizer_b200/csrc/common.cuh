@@ -75,6 +75,14 @@ __device__ __forceinline__ bool accept_linear(float u, float lt, float ld) {
 __device__ __forceinline__ float bf16lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
+// Programmatic dependent launch (launch_overlapped on the host): a kernel starts
+// while the one before it in the stream drains. wait_before() comes before the
+// first access to global memory, reads and writes alike: everything launched
+// before has then completed and is visible. let_next_start() only allows the
+// next kernel's blocks to take free SMs; they wait in turn.
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ uint4 ldg_stream(const void *p) {
     uint4 r;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"

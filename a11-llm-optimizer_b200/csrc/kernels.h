@@ -7,6 +7,26 @@ namespace a11s {
 
 struct StatusWord;
 
+// Launches a kernel that calls wait_before(), overlapped with the one before it
+// in the stream; `cluster` CTAs to a cluster (1: none).
+template <typename... P, typename... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t s, const A &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 struct AcceptArgs {
     const void *target;
     const void *draft;
@@ -195,6 +215,8 @@ struct ChunkAttnArgs {
 };
 cudaError_t launch_chunk_attention_rows(const ChunkAttnArgs &a, cudaStream_t s);
 cudaError_t launch_chunk_attention(const ChunkAttnArgs &a, cudaStream_t s);
+// Zeroes the first `bytes` (a multiple of 4) of the workspace before it.
+cudaError_t launch_chunk_attention_clear(void *workspace, size_t bytes, cudaStream_t s);
 
 struct NormArgs {
     const void *x, *residual, *weight;  // residual: nullable

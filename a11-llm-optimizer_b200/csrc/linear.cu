@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int m0 = (tile % p.m_tiles) * kTileM, n0 = (tile / p.m_tiles) * kOut;
     const int per = (p.slices + p.split - 1) / p.split;
     const int s0 = min(rank * per, p.slices), ns = min(per, p.slices - s0);
-    clear_status(p.status);
+    let_next_start();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
             tc::mbar_init(&bs->full[s], 1);
@@ -281,18 +281,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_alloc(&bs->tmem_base, BN);
         tc::tmem_relinquish();
     }
+    if (warp == 0 && tc::elect_one()) {
+        tc::prefetch_tmap(&tx);
+        tc::prefetch_tmap(&tw);
+        if (GATED) tc::prefetch_tmap(&tg);
+    }
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = bs->tmem_base;
+    wait_before();
+    clear_status(p.status);
 
     if (warp == 0) {
         constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
-        if (tc::elect_one()) {
-            tc::prefetch_tmap(&tx);
-            tc::prefetch_tmap(&tw);
-            if (GATED) tc::prefetch_tmap(&tg);
-        }
         for (int i = 0, s = 0, use = 0; i < ns; ++i) {
             if (use > 0 && !warp_wait(&bs->empty[s], (use - 1) & 1, bs, p.status)) break;
             if (warp_aborted(bs)) break;
@@ -418,8 +420,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int unit = (int)tc::cluster_id(), units = (int)tc::cluster_count();
     const int total = p.m_tiles * p.n_tiles;
     const int my_tiles = unit < total ? (total - 1 - unit) / units + 1 : 0;
-    clear_status(p.status);
-    if (my_tiles == 0) return;  // both CTAs of the pair
+    let_next_start();
+    if (my_tiles == 0) return;  // both CTAs of the pair (the launch has no more pairs than tiles)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) {
@@ -442,6 +444,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     tc::cluster_sync();  // the even CTA's barriers are ready before the peer signals them
     tc::tc_fence_after();
     const uint32_t tmem = bs->tmem_base;
+    wait_before();
+    clear_status(p.status);
 
     if (warp == 0) {
         constexpr int kElems = E4M3 ? kSliceBytes : kSliceBytes / 2;
@@ -732,19 +736,8 @@ cudaError_t launch_tile(const LinearArgs &a, LinParams p, int split, cudaStream_
     auto kernel = linear_tile<E4M3, GATED, BN>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<BN>::kSmem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((long long)p.m_tiles * p.n_tiles * split));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = TileShape<BN>::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, tg, p);
+    return launch_overlapped(kernel, dim3((unsigned)((long long)p.m_tiles * p.n_tiles * split)), kThreads, TileShape<BN>::kSmem,
+                             (unsigned)split, s, tx, tw, tg, p);
 }
 
 // CTA pairs that can be resident at once (one CTA per SM; an odd SM of a group stays out).
@@ -790,8 +783,8 @@ cudaError_t launch_pair(const LinearArgs &a, LinParams p, int sms, cudaStream_t 
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)(2 * std::min<long long>((long long)p.m_tiles * p.n_tiles, pair_slots(kernel, cfg, sms))));
-    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, tg, tout, p);
+    const long long pairs = std::min<long long>((long long)p.m_tiles * p.n_tiles, pair_slots(kernel, cfg, sms));
+    return launch_overlapped(kernel, dim3((unsigned)(2 * pairs)), kPairThreads, kPairSmem, 2, s, tx, tw, tg, tout, p);
 }
 
 template <bool E4M3, bool GATED>

@@ -72,6 +72,8 @@ __global__ void __launch_bounds__(512) linear_skinny_kernel(const SkinnyParams p
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * 16;
+    let_next_start();
+    wait_before();
     if (blockIdx.x == 0 && threadIdx.x == 0 && p.status) *p.status = StatusWord{0, 0};  // nothing here can fail
     // this lane's two weight rows and NT rows of x; absent ones repeat the last (their results are dropped)
     const uint8_t *w[P][2], *x[NT];
@@ -146,8 +148,7 @@ cudaError_t launch_nt(const SkinnyParams &p, cudaStream_t s) {
             const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             if (e != cudaSuccess) return e;
         }
-        kernel<<<blocks, warps * 32, smem, s>>>(p);
-        return cudaGetLastError();
+        return launch_overlapped(kernel, dim3(blocks), warps * 32, smem, 1, s, p);
     };
     switch (nt) {
         case 1: return go(linear_skinny_kernel<E4M3, GATED, 1>);

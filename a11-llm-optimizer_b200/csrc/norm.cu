@@ -110,6 +110,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) add_rms_norm_kernel(const N
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
     const int t = WARP ? lane : threadIdx.x, threads = WARP ? 32 : blockDim.x;
+    let_next_start();
+    wait_before();
     if (WARP && row >= p.rows) return;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
     const T *res = p.residual ? static_cast<const T *>(p.residual) + row * p.res_stride : nullptr;
@@ -230,18 +232,15 @@ cudaError_t launch_vec(const NormParams &p, cudaStream_t s) {
     // 2048 x 2048 and 1 x 2048 (within 2 %).
     constexpr int kFirst = VEC == 1 ? 8 : 1, kLast = 16 / VEC;
     const int vecs = (p.dim + VEC - 1) / VEC;
-    if (vecs <= 32 * kFirst) {
-        add_rms_norm_kernel<T, E4M3, VEC, kFirst, true, PEEL><<<(unsigned)((p.rows + 7ll) / 8), 256, 0, s>>>(p);
-        return cudaGetLastError();
-    }
+    if (vecs <= 32 * kFirst)
+        return launch_overlapped(add_rms_norm_kernel<T, E4M3, VEC, kFirst, true, PEEL>, dim3((unsigned)((p.rows + 7ll) / 8)), 256, 0, 1, s, p);
     int nv = kFirst;
     while (vecs > 1024 * nv) nv *= 2;
     const int threads = ((vecs + nv - 1) / nv + 31) / 32 * 32;
-    if (nv == kFirst) add_rms_norm_kernel<T, E4M3, VEC, kFirst, false, PEEL><<<(unsigned)p.rows, threads, 0, s>>>(p);
-    else if (nv == 2 * kFirst) add_rms_norm_kernel<T, E4M3, VEC, 2 * kFirst, false, PEEL><<<(unsigned)p.rows, threads, 0, s>>>(p);
-    else if (nv <= kLast) add_rms_norm_kernel<T, E4M3, VEC, kLast, false, PEEL><<<(unsigned)p.rows, threads, 0, s>>>(p);
-    else return cudaErrorInvalidValue;
-    return cudaGetLastError();
+    if (nv == kFirst) return launch_overlapped(add_rms_norm_kernel<T, E4M3, VEC, kFirst, false, PEEL>, dim3((unsigned)p.rows), threads, 0, 1, s, p);
+    if (nv == 2 * kFirst) return launch_overlapped(add_rms_norm_kernel<T, E4M3, VEC, 2 * kFirst, false, PEEL>, dim3((unsigned)p.rows), threads, 0, 1, s, p);
+    if (nv <= kLast) return launch_overlapped(add_rms_norm_kernel<T, E4M3, VEC, kLast, false, PEEL>, dim3((unsigned)p.rows), threads, 0, 1, s, p);
+    return cudaErrorInvalidValue;
 }
 
 template <typename T, bool E4M3>
