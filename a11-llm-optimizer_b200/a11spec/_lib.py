@@ -96,6 +96,25 @@ def _load() -> C.CDLL:
 lib = _load()
 
 
+def _load_fast():
+    """a11spec._fast (cpp/fast_ops.cpp), built on the first import where it is missing."""
+    import importlib
+    if not os.path.exists(os.path.join(HERE, "_fast.so")):
+        import importlib.util
+        spec = importlib.util.spec_from_file_location(
+            "_a11spec_build", os.path.join(os.path.dirname(HERE), "build.py"))
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.build_fast()
+    import torch  # noqa: F401  (its libraries first)
+    mod = importlib.import_module("a11spec._fast")
+    mod.set_error_class(A11Error)
+    return mod
+
+
+fast = _load_fast()
+
+
 def check(rc: int) -> None:
     if rc != OK:
         raise A11Error(rc, lib.a11s_last_error().decode())

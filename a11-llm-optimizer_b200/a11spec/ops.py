@@ -7,7 +7,6 @@ torch's caching allocator unless the caller passes one.
 """
 from __future__ import annotations
 
-import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -221,61 +220,11 @@ def lm_head(hidden: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tens
 
 
 # --------------------------------------------------------------------------- K8, K9, K10
-def _rows(t: torch.Tensor, name: str, dim: int, dtype, dev: int):
-    """Element stride between the rows of t [..., dim] on CUDA device `dev`: unit
-    column stride, rows evenly spaced."""
-    shape = t.shape
-    if t.get_device() != dev:
-        raise A11Error(_lib.EINVAL, f"{name} must be on cuda:{dev}")
-    if t.dtype != dtype:
-        raise A11Error(_lib.EINVAL, f"{name} must be {dtype}, got {t.dtype}")
-    if not shape or shape[-1] != dim:
-        raise A11Error(_lib.EINVAL, f"{name} must be [..., {dim}], got {tuple(shape)}")
-    if t.is_contiguous() or t.numel() == 0:
-        return dim
-    stride = t.stride()
-    if stride[-1] != 1 and dim > 1:
-        raise A11Error(_lib.EINVAL, f"{name} must have unit column stride")
-    lead = [(n, s) for n, s in zip(shape[:-1], stride[:-1]) if n != 1]  # an axis of one row has no stride
-    for (_, s), (n, inner) in zip(lead, lead[1:]):
-        if s != inner * n:
-            raise A11Error(_lib.EINVAL, f"{name} rows must be evenly spaced")
-    return lead[-1][1] if lead else dim
-
-
-def _vector(t: Optional[torch.Tensor], name: str, n: int, dtype, dev: int):
-    """Pointer of a dense vector of n elements on CUDA device `dev` (None: null)."""
-    if t is None:
-        return None
-    if t.get_device() != dev or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
-        raise A11Error(_lib.EINVAL, f"{name} must be {n} contiguous {dtype} elements on cuda:{dev}")
-    return t.data_ptr()
-
-
-# the current stream of a device as the C ABI takes it, without a Stream object
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _on_its_device(op):
-    """Runs `op` with the device of its first tensor current."""
-    @functools.wraps(op)
-    def call(first: torch.Tensor, *args, **kw):
-        if not first.is_cuda:
-            raise A11Error(_lib.EINVAL, f"{op.__name__}: CUDA tensors expected")
-        if first.get_device() == torch.cuda.current_device():
-            return op(first, *args, **kw)
-        with torch.cuda.device(first.device):
-            return op(first, *args, **kw)
-    return call
-
-
-_E4M3 = torch.float8_e4m3fn
-_NORM_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
-_LINEAR_TYPES = {torch.bfloat16: _lib.BF16, _E4M3: _lib.E4M3}
+# Checked and called in C++ (cpp/fast_ops.cpp): a decoded token calls them several
+# times per layer. They run on their first tensor's device, on its current stream.
 _ACTIVATIONS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
 
 
-@_on_its_device
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
                  out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
                  scales: Optional[torch.Tensor] = None, sum_out: Optional[torch.Tensor] = None):
@@ -287,44 +236,9 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     for out * scale). h is x + residual rounded to x's type (sum_out when given,
     which may be x or residual itself: in place); None without a residual.
     Tensors may be views whose rows are evenly spaced."""
-    dev, dtype, shape = x.get_device(), x.dtype, x.shape
-    code = _NORM_TYPES.get(dtype)
-    if code is None or not shape or shape[-1] == 0:
-        raise A11Error(_lib.EINVAL, f"add_rms_norm: x must be float32 or bfloat16 [..., dim], got {dtype} {tuple(shape)}")
-    dim, n = shape[-1], x.numel()
-    rows = n // dim
-    xs = _rows(x, "x", dim, dtype, dev)
-    wp = _vector(weight, "weight", dim, dtype, dev)
-    if out is None:
-        out = torch.empty(shape, dtype=out_dtype or dtype, device=x.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise A11Error(_lib.EINVAL, f"add_rms_norm: out is {out.dtype}, out_dtype {out_dtype}")
-    e4m3 = out.dtype == _E4M3
-    os_ = _rows(out, "out", dim, _E4M3 if e4m3 else dtype, dev)
-    if e4m3 and scales is None:
-        scales = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
-    elif scales is not None and not e4m3:
-        raise A11Error(_lib.EINVAL, "add_rms_norm: scales go with e4m3 output")
-    sp = _vector(scales, "scales", rows, torch.float32, dev)
-    rp = hp = None
-    rs = hs = 0
-    same = out.numel() == n
-    if residual is not None:
-        rs, rp = _rows(residual, "residual", dim, dtype, dev), residual.data_ptr()
-        if sum_out is None:
-            sum_out = torch.empty(shape, dtype=dtype, device=x.device)
-        hs, hp = _rows(sum_out, "sum_out", dim, dtype, dev), sum_out.data_ptr()
-        same = same and residual.numel() == n and sum_out.numel() == n
-    elif sum_out is not None:
-        raise A11Error(_lib.EINVAL, "add_rms_norm: sum_out without a residual")
-    if not same:
-        raise A11Error(_lib.EINVAL, "add_rms_norm: x, residual, sum_out and out must have the same rows")
-    check(lib.a11s_add_rms_norm(code, x.data_ptr(), xs, rp, rs, wp, rows, dim, eps, hp, hs,
-                                _lib.E4M3 if e4m3 else code, out.data_ptr(), os_, sp, _raw_stream(dev)))
-    return out, scales, sum_out
+    return _lib.fast.add_rms_norm(x, weight, residual, eps, out_dtype, out, scales, sum_out)
 
 
-@_on_its_device
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
            activation: Optional[str] = None, gate: Optional[torch.Tensor] = None,
            gate_bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -341,48 +255,15 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     or "gelu" (erf). x, out and residual may be views whose rows are evenly
     spaced (x: 16-byte multiples); out may be residual itself. ws (256 bytes)
     receives the status word; check_status=True reads it (and synchronises)."""
-    dev, dtype = x.get_device(), x.dtype
-    if weight.dim() != 2 or x.dim() == 0:
-        raise A11Error(_lib.EINVAL, "linear: x [..., K] and weight [N, K] expected")
-    N, K = weight.shape
-    code = _LINEAR_TYPES.get(dtype)
-    if code is None:
-        raise A11Error(_lib.EINVAL, f"linear: x must be bfloat16 or float8_e4m3fn, got {dtype}")
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise A11Error(_lib.EINVAL, f"linear: activation {activation!r}, not None, 'silu' or 'gelu'")
-    rows = x.numel() // K if K else 0
-    xs = _rows(x, "x", K, dtype, dev)
-    wp = _vector(weight, "weight", N * K, dtype, dev)
-    gp = sx = sw = sg = bp = gbp = rp = None
-    rs = 0
-    if gate is not None:
-        if gate.shape != weight.shape:
-            raise A11Error(_lib.EINVAL, f"linear: gate {tuple(gate.shape)} differs from weight {tuple(weight.shape)}")
-        gp = _vector(gate, "gate", N * K, dtype, dev)
-    if x_scale is not None or weight_scale is not None or gate_scale is not None:
-        sx = _vector(x_scale, "x_scale", rows, torch.float32, dev)
-        sw = _vector(weight_scale, "weight_scale", N, torch.float32, dev)
-        sg = _vector(gate_scale, "gate_scale", N, torch.float32, dev)
-    if bias is not None:
-        bp = _vector(bias, "bias", N, torch.bfloat16, dev)
-    if gate_bias is not None:
-        gbp = _vector(gate_bias, "gate_bias", N, torch.bfloat16, dev)
-    if out is None:
-        out = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=x.device)
-    os_ = _rows(out, "out", N, torch.bfloat16, dev)
-    same = out.numel() == rows * N
-    if residual is not None:
-        rs, rp = _rows(residual, "residual", N, torch.bfloat16, dev), residual.data_ptr()
-        same = same and residual.numel() == rows * N
-    if not same:
-        raise A11Error(_lib.EINVAL, f"linear: out and residual must have x's {rows} rows")
     if ws is None and check_status:
         ws = workspace(256, x.device)
-    check(lib.a11s_linear(code, x.data_ptr(), xs, sx, wp, sw, gp, sg, bp, gbp, rows, K, N, act, rp, rs, out.data_ptr(),
-                          os_, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream(dev)))
+    out = _lib.fast.linear(x, weight, bias, act, gate, gate_bias, residual, x_scale, weight_scale, gate_scale, out, ws)
     if check_status:
-        raise_on_status(ws)
+        with torch.cuda.device(x.device):
+            raise_on_status(ws)
     return out
 
 
@@ -391,7 +272,6 @@ def chunk_attention_workspace_bytes(batch, max_new, num_q_heads, num_kv_heads, h
                                                         max_kv_len))
 
 
-@_on_its_device
 def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
                     ctx_lens: torch.Tensor, n_new: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                     max_kv_len: Optional[int] = None, want_lse: bool = False, out: Optional[torch.Tensor] = None,
@@ -405,44 +285,11 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     bound of ctx_lens[b] + n_new[b] (default: what the page table holds).
     Returns (out, lse, ws); lse [B, n, Hq] fp32 with want_lse, else None. Pass ws
     again to reuse it; calls that overlap on the GPU need one each."""
-    if q.dim() != 4 or k_pool.dim() != 4:
-        raise A11Error(_lib.EINVAL, "chunk_attention: q [B, n, Hq, D] and pools [P, 16, Hkv, D] expected")
-    B, N, Hq, D = q.shape
-    P, pg, Hkv, D2 = k_pool.shape
-    if pg != _lib.PAGE_TOKENS or D2 != D or v_pool.shape != k_pool.shape:
-        raise A11Error(_lib.EINVAL, "pool shape must be [P, 16, Hkv, D] for K and V")
-    dev = q.get_device()
-    stride = q.stride()
-    if q.dtype != torch.bfloat16 or (D > 1 and stride[3] != 1) or (Hq > 1 and stride[2] != D):
-        raise A11Error(_lib.EINVAL, "q must be bfloat16 with a token's heads dense")
-    qs = stride[1] if N > 1 else stride[0] if B > 1 else Hq * D
-    if B > 1 and stride[0] != N * qs:
-        raise A11Error(_lib.EINVAL, "q tokens must be evenly spaced")
-    n_pool, n_q = k_pool.numel(), q.numel()
-    kp = _vector(k_pool, "k_pool", n_pool, torch.bfloat16, dev)
-    vp = _vector(v_pool, "v_pool", n_pool, torch.bfloat16, dev)
-    if page_table.dim() != 2 or page_table.shape[0] != B:
-        raise A11Error(_lib.EINVAL, f"page_table must be [{B}, maxpages], got {tuple(page_table.shape)}")
-    pages = page_table.shape[1]
-    tp = _vector(page_table, "page_table", B * pages, torch.int32, dev)
-    cp = _vector(ctx_lens, "ctx_lens", B, torch.int32, dev)
-    np_ = _vector(n_new, "n_new", B, torch.int32, dev)
-    if max_kv_len is None:
-        max_kv_len = pages * _lib.PAGE_TOKENS
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
-    if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    op = _vector(out, "out", n_q, torch.bfloat16, dev)
-    if want_lse and lse is None:
-        lse = torch.empty(B, N, Hq, dtype=torch.float32, device=q.device)
-    lp = _vector(lse, "lse", B * N * Hq, torch.float32, dev)
-    if ws is None:
-        ws = workspace(chunk_attention_workspace_bytes(B, N, Hq, Hkv, D, max_kv_len), q.device)
-    check(lib.a11s_chunk_attention(q.data_ptr(), qs, kp, vp, P, tp, pages, cp, np_, B, N, Hq, Hkv, D, max_kv_len, scale,
-                                   op, lp, ws.data_ptr(), ws.numel(), _raw_stream(dev)))
+    out, lse, ws = _lib.fast.chunk_attention(q, k_pool, v_pool, page_table, ctx_lens, n_new, scale, max_kv_len,
+                                             bool(want_lse), out, lse, ws)
     if check_status:
-        raise_on_status(ws)
+        with torch.cuda.device(q.device):
+            raise_on_status(ws)
     return out, lse, ws
 
 

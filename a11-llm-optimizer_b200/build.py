@@ -17,6 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT = os.path.join(HERE, "a11spec", "liba11spec.so")
 CPP = os.path.join(HERE, "cpp")
+FAST_OUT = os.path.join(HERE, "a11spec", "_fast.so")
 VERIFIER_OUT = os.path.join(CPP, "libspec_verifier.so")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -79,6 +80,33 @@ def build_verifier(force: bool = False) -> str:
     return VERIFIER_OUT
 
 
+def build_fast(force: bool = False) -> str:
+    """a11spec/_fast.so: the layer operators' argument checks and calls in C++
+    (g++ against this interpreter's and this torch's headers)."""
+    src = os.path.join(CPP, "fast_ops.cpp")
+    hdr = os.path.join(INCLUDE, "a11spec.h")
+    if not force and os.path.exists(FAST_OUT) and all(
+            os.path.getmtime(p) <= os.path.getmtime(FAST_OUT) for p in (src, hdr)):
+        return FAST_OUT
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    lib = os.path.join(root, "lib")
+    inc = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(CUDA_HOME, "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for d in inc:
+        cmd += ["-isystem" if d != INCLUDE else "-I", d]
+    cmd += ["-o", FAST_OUT + ".tmp", src, "-L", os.path.dirname(OUT), "-la11spec", "-Wl,-rpath,$ORIGIN", "-L", lib,
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
+    os.replace(FAST_OUT + ".tmp", FAST_OUT)
+    return FAST_OUT
+
+
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--force", action="store_true")
@@ -86,3 +114,4 @@ if __name__ == "__main__":
     args = ap.parse_args()
     print(build(force=args.force, verbose=args.verbose))
     print(build_verifier(force=args.force))
+    print(build_fast(force=args.force))

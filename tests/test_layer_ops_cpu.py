@@ -98,25 +98,23 @@ def test_wrappers_want_cuda_tensors():
 
 def test_row_strides():
     """The wrappers' row strides: views whose rows are evenly spaced, and nothing else."""
-    from a11spec.ops import _rows
-
-    class Fake:  # a CPU view that says it is on the device
-        def __init__(self, t):
-            self.t = t
-
-        def get_device(self):
-            return 0
-
-        def __getattr__(self, k):
-            return getattr(self.t, k)
-
+    f = _lib.fast.row_stride
     t = torch.zeros(4, 6, 3, 136, dtype=torch.bfloat16)
-    f = lambda v, d: _rows(Fake(v), "x", d, torch.bfloat16, 0)  # noqa: E731
     assert f(t, 136) == 136 and f(t[:, :, 1, :128], 128) == 408 and f(t[:, :1, 1, :128], 128) == 6 * 408
     assert f(t[:1, :1, :1, :128], 128) == 128 and f(t[0, 0, 0, :8], 8) == 8 and f(t[:0], 136) == 136
-    for v in (t[:, 1:3, 1], t.transpose(0, 1)[..., :128], t[..., ::2], t[0, 0, 0, ::2]):
+    for v in (t[:, 1:3, 1], t.transpose(0, 1)[..., :128], t[..., ::2], t[0, 0, 0, ::2], t[0, 0]):
         with pytest.raises(a11spec.A11Error):
-            f(v, v.shape[-1])
+            f(v, v.shape[-1] if v.dim() > 2 or v.stride(-1) > 1 else 8)
+
+
+def test_wrappers_refuse_other_objects():
+    t = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for call in (lambda: a11spec.add_rms_norm([1.0], t), lambda: a11spec.linear(None, t), lambda: a11spec.linear(3, t),
+                 lambda: a11spec.chunk_attention("q", t, t, t, t)):
+        with pytest.raises(a11spec.A11Error, match="tensor"):
+            call()
+    with pytest.raises(a11spec.A11Error, match="activation"):
+        a11spec.linear(t, t, activation="relu")
 
 
 def test_chunk_attention_split_plan():
