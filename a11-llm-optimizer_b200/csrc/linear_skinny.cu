@@ -3,7 +3,7 @@
 //
 // y[m][n] = act(sum_k x[m][k] W[n][k] ...) as in linear.cu. Bound by HBM: N * K
 // weight elements per product; the rows (at most 32) come from L2.
-// A block takes 16 output columns; its warps share the K axis in interleaved
+// A block takes 16 or 32 output columns; its warps share the K axis in interleaved
 // slices of 128 bytes per weight row and add their sums in shared memory, in
 // warp order. With mma.m16n8k16 the 16 weight rows are operand A and 8 rows of
 // x operand B: no lane is wasted on absent rows beyond the 8 of a tile, and a
@@ -11,7 +11,7 @@
 // need M = 128 and the weights in shared memory; here they go from HBM straight
 // into the registers of the instruction that uses them. That works because the
 // order of k inside a slice does not matter as long as A and B agree: a lane
-// loads 16 consecutive bytes of its row, and those are its operands of several
+// loads 32 consecutive bytes of its row, and those are its operands of several
 // instructions.
 // e4m3 values are widened to f16 (exact) for the same instruction: products of
 // two e4m3 values are exact in fp32, as are all but the sums.
@@ -63,73 +63,115 @@ __device__ __forceinline__ void product16(float (&d)[4], const uint4 &w0, const 
         }
     }
 }
+// 32 consecutive bytes, of which those from `left` on are zeros. WIDE: one 32-byte
+// access, so that the four lanes of a row ask for a whole 128-byte line at once.
+struct Bytes32 {
+    uint4 lo, hi;
+};
+// STREAM: read once (the weights); else kept in L1 (x, which the other blocks of
+// the SM read too).
+template <bool WIDE, bool STREAM>
+__device__ __forceinline__ Bytes32 load32(const uint8_t *p, int left) {
+    Bytes32 r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if constexpr (!STREAM) {
+        if (left > 0) r.lo = __ldg(reinterpret_cast<const uint4 *>(p));
+        if (left > 16) r.hi = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+    } else if constexpr (WIDE) {
+        if (left > 0)
+            asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=r"(r.lo.x), "=r"(r.lo.y), "=r"(r.lo.z), "=r"(r.lo.w), "=r"(r.hi.x), "=r"(r.hi.y), "=r"(r.hi.z), "=r"(r.hi.w)
+                         : "l"(p));
+    } else {
+        if (left > 0) r.lo = ldg_stream(p);
+        if (left > 16) r.hi = ldg_stream(p + 16);
+    }
+    return r;
+}
 
-// NT: tiles of 8 rows of x.
-template <bool E4M3, bool GATED, int NT>
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// NT: tiles of 8 rows of x; MT: tiles of 16 weight rows (output columns) of a block.
+template <bool E4M3, bool GATED, int NT, int MT, bool WIDE>
 __global__ void __launch_bounds__(512) linear_skinny_kernel(const SkinnyParams p) {
-    constexpr int P = GATED ? 2 : 1;
-    extern __shared__ float part[];  // [warps][P][NT][16 columns][8 rows]
+    constexpr int P = GATED ? 2 : 1, kCols = 16 * MT;
+    extern __shared__ float part[];  // [warps][P][MT][NT][16 columns][8 rows]
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16;
+    const int n0 = blockIdx.x * kCols;
     let_next_start();
     wait_before();
     if (blockIdx.x == 0 && threadIdx.x == 0 && p.status) *p.status = StatusWord{0, 0};  // nothing here can fail
-    // this lane's two weight rows and NT rows of x; absent ones repeat the last (their results are dropped)
-    const uint8_t *w[P][2], *x[NT];
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            w[i][h] = (i ? p.gate : p.weight) + (int64_t)min(n0 + g + 8 * h, p.N - 1) * p.k_bytes;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) x[j] = p.x + (int64_t)min(8 * j + g, p.rows - 1) * p.x_pitch;
-
-    float acc[P][NT][4] = {};
-    // slices of 128 bytes of k, bytes 16 t and 64 + 16 t of each; k_bytes is a
-    // multiple of 16, so the last slice may end before a lane's bytes
-#pragma unroll(NT <= 2 ? 2 : 1)
-    for (int k0 = warp * 128; k0 < p.k_bytes; k0 += warps * 128) {
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        uint4 a[P][2][2], b[NT][2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int k = k0 + 64 * c + 16 * t;
-            const bool in = k < p.k_bytes;
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) a[i][h][c] = in ? ldg_stream(w[i][h] + k) : zero;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) b[j][c] = in ? __ldg(reinterpret_cast<const uint4 *>(x[j] + k)) : zero;
+    {  // the epilogue's operands into L2 while the weights stream
+        const int c = threadIdx.x % kCols, m = threadIdx.x / kCols, n = n0 + c;
+        if (n < p.N) {
+            if (p.residual && m < p.rows && c == 0) prefetch_l2(p.residual + m * p.res_stride + n);
+            if (m == 0 && c % 8 == 0) {
+                if (p.col.bias) prefetch_l2(p.col.bias + n);
+                if (p.col.w_scale) prefetch_l2(p.col.w_scale + n);
+                if (GATED && p.col.g_bias) prefetch_l2(p.col.g_bias + n);
+                if (GATED && p.col.g_scale) prefetch_l2(p.col.g_scale + n);
+            }
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) product16<E4M3>(acc[i][j], a[i][0][c], a[i][1][c], b[j][c]);
+        if (E4M3 && threadIdx.x == 0) prefetch_l2(p.x_scale);
     }
-    // lane's results: columns n0 + g and n0 + g + 8, rows 8 j + 2 t and + 1
+    // this lane's weight rows and NT rows of x; absent ones repeat the last (their results are dropped)
+    const uint8_t *w[P][MT][2], *x[NT];
 #pragma unroll
     for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            float *d = part + (((warp * P + i) * NT + j) * 16 + g) * 8 + 2 * t;
-            d[0] = acc[i][j][0];
-            d[1] = acc[i][j][1];
-            d[64] = acc[i][j][2];
-            d[65] = acc[i][j][3];
-        }
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                w[i][m][h] = (i ? p.gate : p.weight) + (int64_t)min(n0 + 16 * m + g + 8 * h, p.N - 1) * p.k_bytes + 32 * t;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) x[j] = p.x + (int64_t)min(8 * j + g, p.rows - 1) * p.x_pitch + 32 * t;
+
+    float acc[P][MT][NT][4] = {};
+    // slices of 128 bytes of k, 32 bytes a lane; k_bytes is a multiple of 16, so the
+    // last slice may end before or within a lane's bytes
+#pragma unroll(P * MT * NT <= 2 ? 2 : 1)
+    for (int k0 = warp * 128; k0 < p.k_bytes; k0 += warps * 128) {
+        const int left = p.k_bytes - k0 - 32 * t;
+        Bytes32 a[P][MT][2], b[NT];
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) a[i][m][h] = load32<WIDE, true>(w[i][m][h] + k0, left);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) b[j] = load32<WIDE, false>(x[j] + k0, left);
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    product16<E4M3>(acc[i][m][j], a[i][m][0].lo, a[i][m][1].lo, b[j].lo);
+                    product16<E4M3>(acc[i][m][j], a[i][m][0].hi, a[i][m][1].hi, b[j].hi);
+                }
+    }
+    // lane's results: columns 16 m + g and + 8, rows 8 j + 2 t and + 1
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                float *d = part + ((((warp * P + i) * MT + m) * NT + j) * 16 + g) * 8 + 2 * t;
+                *reinterpret_cast<float2 *>(d) = make_float2(acc[i][m][j][0], acc[i][m][j][1]);
+                *reinterpret_cast<float2 *>(d + 64) = make_float2(acc[i][m][j][2], acc[i][m][j][3]);
+            }
     __syncthreads();
-    for (int o = threadIdx.x; o < NT * 128; o += blockDim.x) {
-        const int c = o & 15, m = o >> 4, n = n0 + c;
+    for (int o = threadIdx.x; o < NT * 8 * kCols; o += blockDim.x) {
+        const int c = o % kCols, m = o / kCols, n = n0 + c;
         if (m >= p.rows || n >= p.N) continue;
-        const float *src = part + ((m >> 3) * 16 + c) * 8 + (m & 7);
+        const float *src = part + (((c >> 4) * NT + (m >> 3)) * 16 + (c & 15)) * 8 + (m & 7);
         float s[2] = {0.0f, 0.0f};
+#pragma unroll 8
         for (int v = 0; v < warps; ++v)
 #pragma unroll
-            for (int i = 0; i < P; ++i) s[i] += src[(v * P + i) * NT * 128];
+            for (int i = 0; i < P; ++i) s[i] += src[(v * P + i) * MT * NT * 128];
         const float xs = E4M3 ? __ldg(p.x_scale + m) : 1.0f;
         float y = finish<GATED>(s[0], s[1], xs, column<GATED>(p.col, n), p.act);
         if (p.residual) y += __bfloat162float(p.residual[m * p.res_stride + n]);
@@ -137,12 +179,22 @@ __global__ void __launch_bounds__(512) linear_skinny_kernel(const SkinnyParams p
     }
 }
 
-template <bool E4M3, bool GATED>
+template <bool E4M3, bool GATED, int NT, bool WIDE>
 cudaError_t launch_nt(const SkinnyParams &p, cudaStream_t s) {
-    const int nt = (p.rows + 7) / 8, blocks = (p.N + 15) / 16;
-    // 8 warps share K; 16 when the blocks alone do not fill the SMs and K has slices for them
-    const int warps = blocks < 148 && p.k_bytes >= 16 * 256 ? 16 : 8;
-    const size_t smem = (size_t)warps * (GATED ? 2 : 1) * nt * 128 * sizeof(float);
+    // Two column tiles a block where that still gives every SM a block and pays:
+    // for a gated product of few rows, gate and weight rows then come in longer runs
+    // (1 x 2048 -> 8192: 13.1 us against 14.2); for more rows x is read half as
+    // often (17 x 2048 -> 5120 e4m3: 7.4 against 8.6; bf16 9.5 against 10.8). Not
+    // for bf16 products of up to 16 rows (9 x 2048 -> 5120: 7.9 against 6.9), gated
+    // ones of more (32 rows: 32 against 20, registers) and e4m3 of over 24 (32 x 2048
+    // -> 5120: 8.7 against 7.4).
+    constexpr bool kTwo = GATED ? NT <= 2 : E4M3 ? NT == 2 || NT == 3 : NT >= 3;
+    const int mt = kTwo && p.N >= 32 * 148 ? 2 : 1;
+    const int blocks = (p.N + 16 * mt - 1) / (16 * mt);
+    // 8 warps share K; 16 when the blocks do not fill the SMs and K has slices for
+    // them (1 x 8192 -> 2048: 10.3 us against 14.7)
+    const int warps = blocks < 148 && p.k_bytes >= 16 * 128 ? 16 : 8;
+    const size_t smem = (size_t)warps * (GATED ? 2 : 1) * mt * NT * 128 * sizeof(float);
     auto go = [&](auto kernel) {
         if (smem > 48 * 1024) {
             const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -150,11 +202,19 @@ cudaError_t launch_nt(const SkinnyParams &p, cudaStream_t s) {
         }
         return launch_overlapped(kernel, dim3(blocks), warps * 32, smem, 1, s, p);
     };
-    switch (nt) {
-        case 1: return go(linear_skinny_kernel<E4M3, GATED, 1>);
-        case 2: return go(linear_skinny_kernel<E4M3, GATED, 2>);
-        case 3: return go(linear_skinny_kernel<E4M3, GATED, 3>);
-        default: return go(linear_skinny_kernel<E4M3, GATED, 4>);
+    if constexpr (kTwo)
+        if (mt == 2) return go(linear_skinny_kernel<E4M3, GATED, NT, 2, WIDE>);
+    return go(linear_skinny_kernel<E4M3, GATED, NT, 1, WIDE>);
+}
+template <bool E4M3, bool GATED>
+cudaError_t launch_type(const SkinnyParams &p, cudaStream_t s) {
+    auto wide = [](const void *ptr, int64_t pitch) { return (reinterpret_cast<uintptr_t>(ptr) & 31) == 0 && pitch % 32 == 0; };
+    const bool w = wide(p.weight, p.k_bytes) && wide(p.gate, 0);
+    switch ((p.rows + 7) / 8) {
+        case 1: return w ? launch_nt<E4M3, GATED, 1, true>(p, s) : launch_nt<E4M3, GATED, 1, false>(p, s);
+        case 2: return w ? launch_nt<E4M3, GATED, 2, true>(p, s) : launch_nt<E4M3, GATED, 2, false>(p, s);
+        case 3: return w ? launch_nt<E4M3, GATED, 3, true>(p, s) : launch_nt<E4M3, GATED, 3, false>(p, s);
+        default: return w ? launch_nt<E4M3, GATED, 4, true>(p, s) : launch_nt<E4M3, GATED, 4, false>(p, s);
     }
 }
 }  // namespace
@@ -177,8 +237,8 @@ cudaError_t launch_linear_skinny(const LinearArgs &a, cudaStream_t s) {
     p.N = a.N;
     p.act = a.act;
     p.status = a.status;
-    if (a.e4m3) return a.gate ? launch_nt<true, true>(p, s) : launch_nt<true, false>(p, s);
-    return a.gate ? launch_nt<false, true>(p, s) : launch_nt<false, false>(p, s);
+    if (a.e4m3) return a.gate ? launch_type<true, true>(p, s) : launch_type<true, false>(p, s);
+    return a.gate ? launch_type<false, true>(p, s) : launch_type<false, false>(p, s);
 }
 
 }  // namespace a11s
