@@ -641,6 +641,9 @@ int a11s_chunk_attention(const void *q, int64_t q_stride, const void *k_pool, co
     if ((double)a.plan.ctiles * batch * a.plan.splits * num_kv_heads > 2147483647.0 ||
         (double)batch * max_new * num_q_heads > 2147483647.0)
         return fail(A11S_EUNSUPPORTED, "a11s_chunk_attention: more rows than a launch holds");
+    if (a.plan.rows && (double)batch * num_kv_heads * max_pages_per_seq > 2e9)
+        return fail(A11S_EUNSUPPORTED, "a11s_chunk_attention: %d sequences x %d KV heads x %d pages are too many for few rows", batch,
+                    num_kv_heads, max_pages_per_seq);
     a.q = q;
     a.q_stride = q_stride;
     a.k_pool = k_pool;

@@ -119,7 +119,7 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 __device__ __forceinline__ int live_tokens(const Params &p, int b, int &ctx, bool tell) {
     ctx = p.ctx_lens[b];
     const int n = p.n_new ? p.n_new[b] : p.N;
-    if (n < 0 || n > p.N || ctx < 0 || (long long)ctx + n > (long long)p.max_pages * A11S_PAGE_TOKENS) {
+    if (n < 0 || n > p.N || ctx < 0 || (long long)ctx + n > min((long long)p.max_pages * A11S_PAGE_TOKENS, (long long)kMaxKv)) {
         if (tell) report(p.status, A11S_EBOUNDS, b);
         ctx = 0;
         return 0;
@@ -577,11 +577,10 @@ cudaError_t launch_chunk_attention_clear(void *workspace, size_t bytes, cudaStre
 }
 
 ChunkPlan chunk_attention_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t max_kv_len) {
-    const int max_pages = (max_kv_len + A11S_PAGE_TOKENS - 1) / A11S_PAGE_TOKENS;
     int sms = 148, dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     ChunkPlan c;
-    if ((long long)N * (Hq / Hkv) <= kChunkRows && B <= kChunkRowsMaxBatch && (double)B * Hkv * max_pages < 1e9) {
+    if ((long long)N * (Hq / Hkv) <= kChunkRows && B <= kChunkRowsMaxBatch) {
         c.rows = true;
         c.splits = chunk_rows_ctas(sms);
         return c;

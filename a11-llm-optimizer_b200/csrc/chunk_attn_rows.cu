@@ -65,7 +65,7 @@ struct Params {
 __device__ __forceinline__ int lengths(const Params &p, int b, int &ctx) {
     ctx = p.ctx_lens[b];
     const int n = p.n_new ? p.n_new[b] : p.N;
-    if (n >= 0 && n <= p.N && ctx >= 0 && (long long)ctx + n <= (long long)p.max_pages * A11S_PAGE_TOKENS) return n;
+    if (n >= 0 && n <= p.N && ctx >= 0 && (long long)ctx + n <= min((long long)p.max_pages * A11S_PAGE_TOKENS, (long long)kMaxKv)) return n;
     ctx = 0;
     return -1;
 }

@@ -191,6 +191,7 @@ struct ChunkPlan {
     int32_t tokens = 1, ctiles = 1, splits = 1, split_blocks = 1;
     bool rows = false;
 };
+constexpr int kMaxKv = 0x7FFFFE00;        // positions of a sequence: block and page rounding stays within 32 bits
 constexpr int kChunkRows = 32;            // tokens x query heads of a KV head up to which the cache is streamed by warps
 constexpr int kChunkRowsMaxBatch = 2048;  // its page sums fit shared memory
 int chunk_rows_ctas(int sms);

@@ -125,7 +125,7 @@ def _linear_ref(x, w, kw, activation):
 
 SIZES = [  # rows, K, N: the streaming kernel, the split tile, the CTA pair; whole and ragged in every direction
     (1, 16, 1), (1, 2048, 48), (7, 48, 17), (8, 208, 100), (13, 4096, 33), (24, 1040, 520), (32, 8192, 16), (32, 272, 1531),
-    (33, 64, 8), (33, 16, 24), (64, 4096, 256), (100, 2064, 200), (128, 1008, 1531), (197, 1008, 515), (300, 512, 2048),
+    (5, 8, 40), (40, 8, 40), (33, 64, 8), (33, 16, 24), (64, 4096, 256), (100, 2064, 200), (128, 1008, 1531), (197, 1008, 515), (300, 512, 2048),
     (2048, 512, 2048), (2049, 144, 4104), (2300, 272, 2055), (4096, 64, 2056), (8200, 32, 1000),
 ]
 
@@ -135,6 +135,8 @@ SIZES = [  # rows, K, N: the streaming kernel, the split tile, the CTA pair; who
 @pytest.mark.parametrize("gated,activation,bias,residual", [(False, None, False, False), (False, "gelu", True, True),
                                                             (True, "silu", False, True), (True, "gelu", True, False)])
 def test_linear(dev, rows, K, N, e4m3, gated, activation, bias, residual):
+    if e4m3 and K % 16:
+        K += 8  # rows of 16-byte multiples
     x, w, kw = _linear_case(rows + 7 * K + 31 * N, rows, K, N, e4m3, gated, bias, residual)
     ref, tol = _linear_ref(x, w, kw, activation)
     out = torch.full((rows, N), math.nan, dtype=BF, device="cuda")
@@ -165,6 +167,10 @@ def test_linear_views_and_in_place_residual(dev, rows):
     y = a11spec.linear(x2, w2, activation="silu", out=odd[:, 1:1 + N], **kw2)
     assert R.worst(y, ref, tol) <= 1
     assert bool((odd[:, :1] == 5).all()) and bool((odd[:, 1 + N:] == 5).all())
+    odd[:, 1:1 + N] = kw2.pop("residual")  # and in place there
+    y = a11spec.linear(x2, w2, activation="silu", residual=odd[:, 1:1 + N], out=odd[:, 1:1 + N], **kw2)
+    assert R.worst(y, ref, tol) <= 1
+    assert bool((odd[:, :1] == 5).all()) and bool((odd[:, 1 + N:] == 5).all())
 
 
 @pytest.mark.parametrize("rows", [3, 70, 2100])
@@ -184,6 +190,19 @@ def test_linear_empty_and_leading_axes(dev):
     x = torch.randn(2, 3, 64, device="cuda").to(BF)
     y = a11spec.linear(x, w)
     assert y.shape == (2, 3, 40) and torch.equal(y.view(6, 40), a11spec.linear(x.view(6, 64), w))
+
+
+def test_linear_outputs_past_32_bits(dev):
+    """More than 2^31 output elements, on even and on odd rows: the last rows are right."""
+    rows, K, N = 66000, 16, 32800
+    g = _gen(77)
+    x, w = _rnd(g, rows, K, dtype=BF), _rnd(g, N, K, dtype=BF)
+    for n in (N, N - 1):
+        y = a11spec.linear(x, w[:n], check_status=True)
+        for lo in (0, 65400, rows - 100):
+            ref, tol = R.linear(x[lo:lo + 100], w[:n])
+            assert R.worst(y[lo:lo + 100], ref, tol) <= 1, (n, lo)
+        del y
 
 
 # --------------------------------------------------------------------------- K10
@@ -245,6 +264,38 @@ def test_chunk_attention_split_caches(dev, ctx, n_new, N, Hq, Hkv, D):
     b, lb, _ = _check_attn(args, max_kv_len=top)
     assert torch.equal(a, b) and torch.equal(la, lb)  # merged in a fixed order
     _check_attn(args, max_kv_len=128)                 # a bound that is too small costs speed only
+
+
+@pytest.mark.parametrize("N", [1, 40])
+def test_chunk_attention_pool_past_32_bits(dev, N):
+    """Pages whose elements lie past 2^31 in the pool."""
+    q, k, v, table, ctx, nn = _cache(14, [700, 90], [N, N], N, 16, 8, 128)
+    big = 140000  # pages of 16 x 8 x 128 elements: 2.29e9
+    kb, vb = (torch.empty(big, 16, 8, 128, dtype=BF, device="cuda") for _ in range(2))
+    shift = big - k.shape[0]
+    kb[shift:], vb[shift:] = k, v
+    moved = torch.where(table >= 0, table + shift, table)
+    want, wl, _ = _check_attn((q, k, v, table, ctx, nn))
+    got, gl, _ = a11spec.chunk_attention(q, kb, vb, moved, ctx, nn, want_lse=True, check_status=True)
+    assert torch.equal(got, want) and torch.equal(gl, wl)
+
+
+def test_chunk_attention_many_sequences(dev):
+    """More sequences than threads of a CTA, most of them short or empty; and more than
+    the few-row kernel's page sums hold."""
+    for B in (700, 2100):
+        ctx = [(b * 37) % 90 if b % 5 else 0 for b in range(B)]
+        nn = [1 if b % 3 else 0 for b in range(B)]
+        args = _cache(15, ctx, nn, 1, 4, 2, 64)
+        a, la, _ = _check_attn(args)
+        b, lb, _ = _check_attn(args)
+        assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+def test_chunk_attention_one_long_among_short(dev):
+    """Shares cut the long sequence many times and hold many short ones whole."""
+    ctx = [30000] + [20 + 3 * b for b in range(60)]
+    _check_attn(_cache(16, ctx, [1] * 61, 1, 8, 2, 128))
 
 
 def test_chunk_attention_default_lengths_and_scale(dev):
