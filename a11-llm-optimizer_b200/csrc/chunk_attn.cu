@@ -508,16 +508,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Merge of the splits of each live row, in split order: one block of D threads
-// per (b, token, head); the splits' weights first, one per thread.
+// Merge of the splits of each live row, in split order: one warp per (b, token,
+// head); the splits' weights first, one or two per lane.
 template <int D>
-__global__ void __launch_bounds__(D) chunk_attn_combine(const Params p) {
-    __shared__ float weight[kMaxSplits];
-    __shared__ float total[2];
-    const size_t row = blockIdx.x, rows = (size_t)p.B * p.N * p.Hq;
+__global__ void __launch_bounds__(256) chunk_attn_combine(const Params p) {
+    constexpr int W = D / 32;  // dims of a lane
+    const size_t row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (size_t)p.B * p.N * p.Hq;
     let_next_start();
     wait_before();
-    const int t = threadIdx.x, b = (int)(row / ((size_t)p.N * p.Hq)), token = (int)((row / p.Hq) % p.N);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 31, b = (int)(row / ((size_t)p.N * p.Hq)), token = (int)((row / p.Hq) % p.N);
     int L;
     const int n_live = live_tokens(p, b, L, false);
     if (token >= n_live) return;  // its zeros are written
@@ -525,42 +525,47 @@ __global__ void __launch_bounds__(D) chunk_attn_combine(const Params p) {
     const int per_cta = kTiles * p.tokens, last = min(n_live, (token / per_cta + 1) * per_cta) - 1;
     const int nblk = (L + last + kBlockKV) / kBlockKV;
     const int splits = min(p.splits, (nblk + p.split_blocks - 1) / p.split_blocks);
-    const float *po = p.part_o + row * D + t;
-    if (t < 32) {  // weights 2^(m - M) l and their sum (each split's output is already divided by its l)
-        float m[kMaxSplits / 32], l[kMaxSplits / 32], M = -INFINITY, sum = 0.0f;
+    // weights 2^(m - M) l over their sum (each split's output is already divided by its l)
+    float m[kMaxSplits / 32], w[kMaxSplits / 32], M = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kMaxSplits / 32; ++i) {
-            const int s = t + 32 * i;
-            const size_t at = ((size_t)min(s, splits - 1) * rows + row) * 2;
-            m[i] = p.part_ml[at];
-            l[i] = s < splits ? p.part_ml[at + 1] : 0.0f;
-            if (l[i] != 0.0f) M = fmaxf(M, m[i]);
-        }
-        M = warp_fmax(M);
-#pragma unroll
-        for (int i = 0; i < kMaxSplits / 32; ++i) {
-            const float w = l[i] == 0.0f ? 0.0f : l[i] * exp2f(m[i] - M);
-            weight[t + 32 * i] = w;
-            sum += w;
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (t == 0) {
-            total[0] = sum;
-            total[1] = M;
-        }
+    for (int i = 0; i < kMaxSplits / 32; ++i) {
+        const int s = lane + 32 * i;
+        const size_t at = ((size_t)min(s, splits - 1) * rows + row) * 2;
+        m[i] = p.part_ml[at];
+        w[i] = s < splits ? p.part_ml[at + 1] : 0.0f;
+        if (w[i] != 0.0f) M = fmaxf(M, m[i]);
     }
-    __syncthreads();
-    float acc = 0.0f;
-#pragma unroll 16
+    M = warp_fmax(M);
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; ++i) {
+        w[i] = w[i] == 0.0f ? 0.0f : w[i] * exp2f(m[i] - M);
+        sum += w[i];
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float *po = p.part_o + row * D + lane * W;
+    float acc[W] = {};
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) {
-        const float w = weight[s], o = po[(size_t)s * rows * D];
-        if (w != 0.0f) acc = fmaf(w, o, acc);
+        const float f = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[kMaxSplits / 32 - 1], s & 31);
+        float o[W];
+        if constexpr (W == 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(po + (size_t)s * rows * D);
+            o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2 *>(po + (size_t)s * rows * D);
+            o[0] = v.x, o[1] = v.y;
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) acc[e] = fmaf(f, f == 0.0f ? 0.0f : o[e], acc[e]);  // a split that saw nothing takes no part
     }
-    const float sum = total[0], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    p.out[row * D + t] = __float2bfloat16_rn(acc * inv);
-    if (p.lse && t == 0) p.lse[row] = sum == 0.0f ? 0.0f : (total[1] + log2f(sum)) * 0.6931471805599453f;
+    uint32_t *out = reinterpret_cast<uint32_t *>(p.out + row * D + lane * W);
+#pragma unroll
+    for (int e = 0; e < W; e += 2) out[e / 2] = tc::cvt_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+    if (p.lse && lane == 0) p.lse[row] = sum == 0.0f ? 0.0f : (M + log2f(sum)) * 0.6931471805599453f;
 }
+static_assert(kMaxSplits == 64, "two weights per lane");
 
 // ---------------------------------------------------------------------------- host side
 // Clears the status word and the merge counters: a kernel and not a memset, so
@@ -650,7 +655,7 @@ cudaError_t launch_d(const ChunkAttnArgs &a, const Params &p, cudaStream_t s) {
     e = launch_overlapped(kernel, dim3((unsigned)((long long)p.ctiles * p.B * p.splits * p.Hkv)), kThreads, Shape<D>::kSmem, 1, s,
                           tk, tv, p);
     if (e != cudaSuccess || p.splits == 1) return e;
-    return launch_overlapped(chunk_attn_combine<D>, dim3((unsigned)((size_t)p.B * p.N * p.Hq)), D, 0, 1, s, p);
+    return launch_overlapped(chunk_attn_combine<D>, dim3((unsigned)(((size_t)p.B * p.N * p.Hq + 7) / 8)), 256, 0, 1, s, p);
 }
 }  // namespace
 
