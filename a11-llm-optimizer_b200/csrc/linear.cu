@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const uint32_t srow = tc::smem_u32(box) + (uint32_t)lane * 64u;
         const bool params = p.col.any();
         bool ok = true;
-        for (int i = 0; i < my_tiles && ok; ++i) {
+        for (int i = 0; i < my_tiles; ++i) {  // to the end also after a timeout: the warps meet at a barrier
             const int t = unit + i * units;
             const int mw = (t % p.m_tiles) * kPairM + (int)rank * 128 + q * 32, n0 = (t / p.m_tiles) * kOut;
             const int buf = i & 1, m = mw + lane;
@@ -540,6 +540,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 stage_columns<GATED, kOut>(cols, p.col, n0, p.N, threadIdx.x - 64, kEpiThreads);
                 epilogue_barrier<kEpiThreads>();
             }
+            if (!ok) continue;
             if (E4M3 && m < p.rows) xs = __ldg(p.x_scale + m);
             uint4 res[4];
             auto load_residual = [&](int n) {  // this row's 32 columns at n; absent ones are never stored
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             };
             if (p.vec_res) load_residual(n0 + first * kEpiCols);
             ok = warp_wait(&bs->acc_full[buf], (i >> 1) & 1, bs, p.status);
-            if (!ok) break;
+            if (!ok) continue;
             tc::tc_fence_after();
 #pragma unroll 1
             for (int h = first; h < kSteps; h += 2) {
