@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int lp_end = min((kv_len + A11S_PAGE_TOKENS - 1) / A11S_PAGE_TOKENS, (blk0 + nb) * kPagesPerBlock);
             auto window = [&](int w) -> int {
                 const int lp = lp0 + 32 * w + lane;
-                return lp < lp_end ? __ldg(pt + lp) : -2;
+                return lp < lp_end ? pt[lp] : -2;
             };
             int cur = window(0), nxt = window(1);
             int nk = 0, nv = 0;
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint4 *src = reinterpret_cast<const uint4 *>(p.q + ((int64_t)b * p.N + token) * p.q_stride + head * D);
 #pragma unroll
                 for (int c = 0; c < kQ16; ++c) {
-                    const uint4 v = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+                    const uint4 v = live ? src[c] : make_uint4(0, 0, 0, 0);
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                     tc::st_shared_v4(q_row + (uint32_t)(c >> 3) * kHalf + ((uint32_t)((c & 7) ^ (m & 7)) << 4), w);
                 }

@@ -181,13 +181,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_rows(const Params p) {
         if (count > 0) {
             const int mine = (count - warp + kWarps - 1) / kWarps;  // pages first + warp, + 8, ...
             const int32_t *table = p.page_table + (size_t)b * p.max_pages + first + warp;
-            int ids = lane < mine ? __ldg(table + kWarps * lane) : 0;  // page ids of 32 of the warp's pages, from ids0 on
+            int ids = lane < mine ? table[kWarps * lane] : 0;  // page ids of 32 of the warp's pages, from ids0 on
             int ids0 = 0;
             auto issue = [&](int i) {  // K and V of the warp's page i into its ring slot
                 if (i < mine) {
                     if (i - ids0 >= 32) {
                         ids0 += 32;
-                        ids = ids0 + lane < mine ? __ldg(table + kWarps * (ids0 + lane)) : 0;
+                        ids = ids0 + lane < mine ? table[kWarps * (ids0 + lane)] : 0;
                     }
                     int id = __shfl_sync(0xffffffffu, ids, i - ids0);
                     const bool good = id >= 0 && id < p.num_pages;
@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attn_rows(const Params p) {
                 const __nv_bfloat16 *src = p.q + ((int64_t)b * p.N + (in ? token : 0)) * p.q_stride + (g * p.group + (in ? r % p.group : 0)) * D;
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
-                    qf[j][s][0] = in ? __ldg(reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * t4)) : 0u;
-                    qf[j][s][1] = in ? __ldg(reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * t4)) : 0u;
+                    qf[j][s][0] = in ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * t4) : 0u;
+                    qf[j][s][1] = in ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * t4) : 0u;
                 }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {

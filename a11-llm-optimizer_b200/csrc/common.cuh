@@ -79,9 +79,21 @@ __device__ __forceinline__ float bf16hi(uint32_t w) { return __uint_as_float(w &
 // while the one before it in the stream drains. wait_before() comes before the
 // first access to global memory, reads and writes alike: everything launched
 // before has then completed and is visible. let_next_start() only allows the
-// next kernel's blocks to take free SMs; they wait in turn.
+// next kernel's blocks to take free SMs; they wait in turn. What such a kernel
+// reads may be written by the one before it, within its own lifetime: its loads
+// are coherent ones (ld_stream, plain loads), never ld.global.nc or __ldg, which
+// the compiler may move up over the wait and whose cached lines need not be fresh.
 __device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// 16 bytes that are read once, past L1.
+__device__ __forceinline__ uint4 ld_stream(const void *p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+    return r;
+}
 
 __device__ __forceinline__ uint4 ldg_stream(const void *p) {
     uint4 r;

@@ -43,11 +43,11 @@ struct Column {
 template <bool GATED>
 __device__ __forceinline__ Column column(const ColumnParams &p, int n) {
     Column c{1.0f, 0.0f, 1.0f, 0.0f};
-    if (p.w_scale) c.w_scale = __ldg(p.w_scale + n);
-    if (p.bias) c.bias = __bfloat162float(__ldg(p.bias + n));
+    if (p.w_scale) c.w_scale = p.w_scale[n];
+    if (p.bias) c.bias = __bfloat162float(p.bias[n]);
     if (GATED) {
-        if (p.g_scale) c.g_scale = __ldg(p.g_scale + n);
-        if (p.g_bias) c.g_bias = __bfloat162float(__ldg(p.g_bias + n));
+        if (p.g_scale) c.g_scale = p.g_scale[n];
+        if (p.g_bias) c.g_bias = __bfloat162float(p.g_bias[n]);
     }
     return c;
 }

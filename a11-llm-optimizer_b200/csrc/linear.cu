@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool params = p.col.any();
         if (params) {
             stage_columns<GATED, kOut>(cols_sm, p.col, n0, p.N, t, 128);
-            xs_sm[t] = E4M3 && m0 + t < p.rows ? __ldg(p.x_scale + m0 + t) : 1.0f;
+            xs_sm[t] = E4M3 && m0 + t < p.rows ? p.x_scale[m0 + t] : 1.0f;
         }
         epilogue_barrier<128>();
         auto run = [&](auto split) {
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 epilogue_barrier<kEpiThreads>();
             }
             if (!ok) continue;
-            if (E4M3 && m < p.rows) xs = __ldg(p.x_scale + m);
+            if (E4M3 && m < p.rows) xs = p.x_scale[m];
             uint4 res[4];
             auto load_residual = [&](int n) {  // this row's 32 columns at n; absent ones are never stored
                 const bool in = m < p.rows;

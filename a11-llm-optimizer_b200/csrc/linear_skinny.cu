@@ -76,16 +76,16 @@ template <bool WIDE, bool STREAM>
 __device__ __forceinline__ Bytes32 load32(const uint8_t *p, int left) {
     Bytes32 r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     if constexpr (!STREAM) {
-        if (left > 0) r.lo = __ldg(reinterpret_cast<const uint4 *>(p));
-        if (left > 16) r.hi = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+        if (left > 0) r.lo = *reinterpret_cast<const uint4 *>(p);
+        if (left > 16) r.hi = reinterpret_cast<const uint4 *>(p)[1];
     } else if constexpr (WIDE) {
         if (left > 0)
-            asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+            asm volatile("ld.global.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                          : "=r"(r.lo.x), "=r"(r.lo.y), "=r"(r.lo.z), "=r"(r.lo.w), "=r"(r.hi.x), "=r"(r.hi.y), "=r"(r.hi.z), "=r"(r.hi.w)
                          : "l"(p));
     } else {
-        if (left > 0) r.lo = ldg_stream(p);
-        if (left > 16) r.hi = ldg_stream(p + 16);
+        if (left > 0) r.lo = ld_stream(p);
+        if (left > 16) r.hi = ld_stream(p + 16);
     }
     return r;
 }
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(512) linear_skinny_kernel(const SkinnyParams p
         for (int v = 0; v < warps; ++v)
 #pragma unroll
             for (int i = 0; i < P; ++i) s[i] += src[(v * P + i) * MT * NT * 128];
-        const float xs = E4M3 ? __ldg(p.x_scale + m) : 1.0f;
+        const float xs = E4M3 ? p.x_scale[m] : 1.0f;
         float y = finish<GATED>(s[0], s[1], xs, column<GATED>(p.col, n), p.act);
         if (p.residual) y += __bfloat162float(p.residual[m * p.res_stride + n]);
         p.out[m * p.out_stride + n] = __float2bfloat16_rn(y);

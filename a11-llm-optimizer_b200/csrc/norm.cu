@@ -51,12 +51,24 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return d;
 }
 
+// One element. As ld_stream, free to move over the stores, which it never aliases
+// before its own element's; not over wait_before().
+__device__ __forceinline__ float ld_one(const float *p) {
+    float f;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(f) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ float ld_one(const __nv_bfloat16 *p) {
+    uint16_t u;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(u) : "l"(p));
+    return bf16lo(u);
+}
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T *p, float (&f)[VEC]) {
     if constexpr (VEC == 1) {
-        f[0] = (float)__ldg(p);
+        f[0] = ld_one(p);
     } else if constexpr (sizeof(T) == 2) {
-        const uint4 u = ldg_stream(p);
+        const uint4 u = ld_stream(p);
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -64,7 +76,7 @@ __device__ __forceinline__ void load_vec(const T *p, float (&f)[VEC]) {
             f[2 * i + 1] = bf16hi(w[i]);
         }
     } else {
-        const uint4 u = ldg_stream(p);
+        const uint4 u = ld_stream(p);
         f[0] = __uint_as_float(u.x);
         f[1] = __uint_as_float(u.y);
         f[2] = __uint_as_float(u.z);
@@ -156,14 +168,14 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) add_rms_norm_kernel(const N
     for (int i = 0; i < NV; ++i) {
         const int c = (i * threads + t) * VEC;
         if (c < body) {
-            if (sum) store_vec<T, VEC>(sum + head + c, h[i]);
             float w[VEC];
             if constexpr (PEEL) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) w[e] = (float)__ldg(wt + head + c + e);
+                for (int e = 0; e < VEC; ++e) w[e] = ld_one(wt + head + c + e);
             } else {
                 load_vec<T, VEC>(wt + c, w);
             }
+            if (sum) store_vec<T, VEC>(sum + head + c, h[i]);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 ss = fmaf(h[i][e], h[i][e], ss);
@@ -176,7 +188,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) add_rms_norm_kernel(const N
         const float one[1] = {he};
         if (sum) store_vec<T, 1>(sum + extra, one);
         ss = fmaf(he, he, ss);
-        he *= (float)__ldg(wt + extra);
+        he *= ld_one(wt + extra);
         if (E4M3) mx = max_nan(mx, fabsf(he));
     }
 #pragma unroll

@@ -406,3 +406,72 @@ def test_layers_on_two_streams(dev):
             gb = [_layer(b) for _ in range(3)]
         torch.cuda.synchronize()
         assert all(torch.equal(x, wa) for x in ga) and all(torch.equal(x, wb) for x in gb)
+
+
+def _chain(s, steps, each=lambda: None):
+    """Norm, gated product, product, each writing what the next and the one after the next read."""
+    for _ in range(steps):
+        a11spec.add_rms_norm(s["h"], s["w"], residual=s["d"], sum_out=s["h"], out=s["y"])
+        each()
+        a11spec.linear(s["y"], s["up"], gate=s["gate"], activation="silu", out=s["a"])
+        each()
+        a11spec.linear(s["a"], s["down"], bias=s["bias"], out=s["d"])
+        each()
+        s["bias"].copy_(s["d"][0])  # a parameter that another library's kernel writes between calls
+        each()
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 512), (20, 512), (70, 264), (300, 2048)])
+def test_calls_in_a_row_see_each_others_results(dev, rows, dim):
+    """Kernels that start over the tail of the one before read what it wrote:
+    run together or captured, a chain in the same buffers gives the bits that it gives
+    with a synchronisation after each call."""
+    g = _gen(rows)
+    s = dict(w=_rnd(g, dim, std=0.5, dtype=BF), up=_rnd(g, 2 * dim, dim, std=dim ** -0.5, dtype=BF), bias=_rnd(g, dim, dtype=BF),
+             gate=_rnd(g, 2 * dim, dim, std=dim ** -0.5, dtype=BF), down=_rnd(g, dim, 2 * dim, std=dim ** -0.5, dtype=BF),
+             h=_rnd(g, rows, dim, dtype=BF), d=_rnd(g, rows, dim, dtype=BF))
+    s["y"], s["a"] = torch.empty_like(s["h"]), torch.empty(rows, 2 * dim, device="cuda", dtype=BF)
+    start = {k: s[k].clone() for k in ("h", "d", "bias")}
+
+    def run(f):
+        for k, v in start.items():
+            s[k].copy_(v)
+        f()
+        torch.cuda.synchronize()
+        return torch.cat([s["h"], s["d"]]).clone()
+
+    want = run(lambda: _chain(s, 40, torch.cuda.synchronize))
+    assert bool(want.isfinite().all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _chain(s, 40)
+    for _ in range(4):
+        assert torch.equal(run(lambda: _chain(s, 40)), want)
+        assert torch.equal(run(graph.replay), want)
+
+
+@pytest.mark.parametrize("N", [1, 40])
+def test_graph_with_a_fork_and_a_join(dev, N):
+    """Two layers on forked streams in one graph, their results added after the join."""
+    a, b = _layer_state(24, 2, N), _layer_state(25, 2, N)
+    h0 = b["h"].clone()
+
+    def both(side):
+        x = _layer(a)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            y = _layer(b)
+        z = _layer(dict(a, h=x))
+        torch.cuda.current_stream().wait_stream(side)
+        return _layer(dict(a, h=a11spec.add_rms_norm(z, a["w_norm"], residual=y)[0])), y
+
+    b["h"] = h0 * 2
+    want = [t.clone() for t in both(torch.cuda.Stream())]
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        out = both(side)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
