@@ -234,7 +234,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     Returns (y, scales, h). y has out_dtype (default: out's type, else x's): x's
     type, or torch.float8_e4m3fn with `scales` fp32 [...], one per row (y stands
     for out * scale). h is x + residual rounded to x's type (sum_out when given,
-    which may be x or residual itself: in place); None without a residual.
+    which may be x or residual itself: in place); None without a residual. out
+    overlaps none of the other tensors.
     Tensors may be views whose rows are evenly spaced."""
     return _lib.fast.add_rms_norm(x, weight, residual, eps, out_dtype, out, scales, sum_out)
 
@@ -253,8 +254,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     (x_scale [...]) and of the weights (weight_scale, gate_scale [N]): what
     add_rms_norm(out_dtype=torch.float8_e4m3fn) gives. activation: None, "silu"
     or "gelu" (erf). x, out and residual may be views whose rows are evenly
-    spaced (x: 16-byte multiples); out may be residual itself. ws (256 bytes)
-    receives the status word; check_status=True reads it (and synchronises)."""
+    spaced (x: 16-byte multiples); out may be residual itself and overlaps nothing
+    else. ws (256 bytes) receives the status word; check_status=True reads it (and
+    synchronises)."""
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise A11Error(_lib.EINVAL, f"linear: activation {activation!r}, not None, 'silu' or 'gelu'")
@@ -283,7 +285,8 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     page_table [B, maxpages]. Token i < n_new[b] (default n) sees positions
     0 .. ctx_lens[b] + i; the other rows come back as zeros. max_kv_len: an upper
     bound of ctx_lens[b] + n_new[b] (default: what the page table holds).
-    Returns (out, lse, ws); lse [B, n, Hq] fp32 with want_lse, else None. Pass ws
+    Returns (out, lse, ws); lse [B, n, Hq] fp32 with want_lse, else None; out
+    overlaps no input. Pass ws
     again to reuse it; calls that overlap on the GPU need one each."""
     out, lse, ws = _lib.fast.chunk_attention(q, k_pool, v_pool, page_table, ctx_lens, n_new, scale, max_kv_len,
                                              bool(want_lse), out, lse, ws)

@@ -727,6 +727,9 @@ int a11s_linear(int32_t dtype, const void *x, int64_t x_stride, const float *x_s
     if (dtype != A11S_BF16 && dtype != A11S_E4M3) return fail(A11S_EINVAL, "a11s_linear: dtype %d", dtype);
     const int per16 = dtype == A11S_E4M3 ? 16 : 8;
     if (rows < 0 || in_dim < 1 || out_dim < 1) return fail(A11S_EINVAL, "a11s_linear: bad sizes");
+    if (rows > A11S_LINEAR_MAX || out_dim > A11S_LINEAR_MAX || in_dim > A11S_LINEAR_MAX / 2)
+        return fail(A11S_EUNSUPPORTED, "a11s_linear: %d x %d -> %d is beyond %d rows or columns, or half as many in_dim", rows,
+                    in_dim, out_dim, A11S_LINEAR_MAX);
     if (in_dim % per16 || x_stride % per16)
         return fail(A11S_EINVAL, "a11s_linear: in_dim and x_stride must be multiples of %d (16 bytes)", per16);
     if (x_stride < in_dim || out_stride < out_dim || (residual && residual_stride < out_dim))

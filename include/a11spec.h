@@ -345,11 +345,13 @@ int a11s_add_rms_norm(int32_t dtype, const void *x, int64_t x_stride, const void
  * apart (nullable); out bf16, rows out_stride apart, may be residual itself but
  * overlap no other input. activation: A11S_ACT_*.
  * in_dim and x_stride multiples of 16 bytes, x, weight and gate 16-byte aligned;
- * rows, out_dim, out_stride and residual_stride are free. The order of the sum
+ * rows and out_dim up to A11S_LINEAR_MAX (in_dim up to half of it), out_stride and
+ * residual_stride are free. The order of the sum
  * over in_dim is fixed by the sizes: equal calls give equal bits.
  * workspace (nullable, >= 256 bytes): the status word, A11S_ETIMEOUT if a
  * pipeline wait of the kernel ran out; without it that is not reported.
  */
+#define A11S_LINEAR_MAX (1 << 30)
 int a11s_linear(int32_t dtype, const void *x, int64_t x_stride, const float *x_scale, const void *weight,
                 const float *weight_scale, const void *gate, const float *gate_scale, const void *bias,
                 const void *gate_bias, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t activation,

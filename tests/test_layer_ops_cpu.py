@@ -124,3 +124,9 @@ def test_chunk_attention_split_plan():
     assert f(1, 4096, 32, 4, 128, 16384) == 256
     assert f(1, 1, 32, 4, 128, 32768) > 256
     assert f(0, 1, 32, 4, 128, 64) == 256 and f(1, 0, 32, 4, 128, 64) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(rows=2 ** 30 + 1), dict(N=2 ** 30 + 8, os=2 ** 30 + 8), dict(K=2 ** 29 + 8, xs=2 ** 29 + 8),
+                                dict(K=2 ** 30, xs=2 ** 30, N=1, os=1, **E4)])
+def test_linear_refuses_sizes_beyond_32_bit_offsets(kw):
+    _refused(_linear(**kw), _lib.EUNSUPPORTED, "beyond")
