@@ -32,12 +32,13 @@
 // exceeds it by more than 8 (log2 units), so exponents stay below 2^8.
 // V rows past the last visible position are zeroed in shared memory: whatever
 // the page holds there (a probability of 0 times a NaN would be NaN).
-// Measured (one B200): 4096 tokens over 12288 (32 / 4 heads of 128) 919 us =
-// 1.05 PFLOP/s; 4 x 300 over up to 2000 (24 / 8 heads of 64) 37.8 us. A softmax warp
+// Measured (one B200): 4096 tokens over 12288 (32 / 4 heads of 128) 920 to
+// 935 us = 1.03 PFLOP/s; 4 x 300 over up to 2000 (24 / 8 heads of 64) 37.8 us. A softmax warp
 // spends about 2750 cycles on a block, 1400 of them on the exponentials, and two
 // warps share a scheduler and its MUFU: the barriers it waits at are already
-// complete. Polling them ahead of time, or one tile per CTA with two CTAs per SM
-// at D = 64, measured slower (941 us; 55 us).
+// complete. Measured slower: polling them ahead of time (941 us), one tile per CTA
+// with two CTAs per SM at D = 64 (55 us), a quarter of the exponentials as a
+// polynomial on the FMA units (983 us), two threads a row (1785 us, spills).
 // Every mbarrier wait is bounded (clock budget); a timeout sets ETIMEOUT and
 // the CTA drains and returns.
 #include <cuda.h>

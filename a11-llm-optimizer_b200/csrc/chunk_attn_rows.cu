@@ -22,8 +22,8 @@
 // sequences (16 pages on average or less) stay whole.
 // Tokens past the last visible one are never read: their copies are zero-filled.
 // Measured (one B200): 32 sequences of one token over up to 4096 (32 / 4 heads of
-// 128, 200 MB) 40.4 us = 4.9 TB/s, 61 through chunk_attn_tc; one token over 32767
-// (67 MB, 37 pieces per KV head) 23.6 us, 33 through chunk_attn_tc with 64 splits.
+// 128, 200 MB) 41 us = 4.9 TB/s, 61 through chunk_attn_tc; one token over 32767
+// (67 MB, 37 pieces per KV head) 23.7 us, 33 through chunk_attn_tc with 64 splits.
 #include <algorithm>
 
 #include "common.cuh"

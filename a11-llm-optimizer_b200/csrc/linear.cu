@@ -18,8 +18,8 @@
 //                 added in rank order.
 //   linear_pair   persistent CTA pairs (cta_group::2), 256 x 256 tiles: sizes
 //                 that fill the GPU. Tensor-bound; structure as in lm_head.cu.
-// Measured (one B200): 2048 x 8192 -> 2048 59 us = 1.16 PFLOP/s (64 tiles on 74
-// pairs), 8192 x 2048 -> 8192 gated e4m3 236 us = 2.33 PFLOP/s (10.5 TB/s of operands
+// Measured (one B200): 2048 x 8192 -> 2048 60 us = 1.14 PFLOP/s (64 tiles on 74
+// pairs), 8192 x 2048 -> 8192 gated e4m3 237 to 242 us = 2.3 PFLOP/s (10.4 TB/s of operands
 // from L2 into the SMs), 197 x 1000 -> 1531 9.4 us, 64 x 8192 -> 2048 14.5 us.
 // A gated product takes gate and weight rows side by side in one tile (half the
 // columns each), so x is staged once for both and act(u) v is formed from two

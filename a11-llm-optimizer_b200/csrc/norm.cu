@@ -22,8 +22,8 @@
 // from a 16-byte boundary: the body is moved in vectors from the first boundary
 // on, and the up to 2 x 7 elements before and after it by one thread each.
 // Where the tensors differ in that distance, every access is one element.
-// Measured (one B200): 8190 x 4999 fp32 104 us = 6.3 TB/s (188 with one element per
-// access), 2048 x 2048 bf16 to e4m3 6.6 us, one row of 2048 2.6 us.
+// Measured (one B200): 8190 x 4999 fp32 104 to 109 us = 6.0 to 6.3 TB/s (188 with one element per
+// access), 2048 x 2048 bf16 to e4m3 6.5 us, one row of 2048 2.6 us.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
