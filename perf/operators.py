@@ -261,19 +261,12 @@ def _plain_attn(s):
     return out
 
 
-_package = None
-
-
 def _a11spec():
-    """The package, imported once as a program does."""
-    global _package
-    if _package is None:
-        pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "a11-llm-optimizer_b200")
-        if pkg not in sys.path:
-            sys.path.insert(0, pkg)
-        import a11spec
-        _package = a11spec
-    return _package
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "a11-llm-optimizer_b200")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import a11spec
+    return a11spec
 
 
 def run(state):
