@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import a11spec
+from test_layer_ops_gpu import _cache, _check_attn
 
 pytestmark = pytest.mark.gpu
 BF, F32, E4 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
@@ -45,3 +46,33 @@ def test_norm_e4m3_follows_its_own_fp32_output(dev, rows, dim, magnitude):
     top = y.abs().amax(1)
     assert torch.equal(s, top / torch.full_like(top, 448.0))
     assert torch.equal(q.float(), (y / s[:, None].expand_as(y)).to(E4).float())
+
+
+# --------------------------------------------------------------------------- K10
+def _pieces(ws, B, Hkv):
+    """Pieces that each (sequence, KV head) was cut into: the merge counters behind the status word (256 bytes)."""
+    return ws[256:256 + 4 * B * Hkv].view(torch.int32).view(B, Hkv)
+
+
+@pytest.mark.parametrize("slots,long_at,ctx,short,Hq,Hkv,D", [(64, 5, 15000, 0, 32, 4, 128), (256, 255, 60000, 0, 8, 1, 64),
+                                                              (200, 0, 12000, 20, 4, 2, 64)])
+def test_one_long_sequence_among_empty_slots_is_cut(dev, slots, long_at, ctx, short, Hq, Hkv, D):
+    """A padded batch of single tokens: many slots are empty or short, one sequence is long.
+    The average over the slots is below 16 pages; the long sequence's pages are still
+    shared by many CTAs."""
+    lens = [short + b % 3 if short else 0 for b in range(slots)]
+    new = [1 if short else 0] * slots
+    lens[long_at], new[long_at] = ctx, 1
+    assert sum((c + n + 15) // 16 for c, n in zip(lens, new)) <= 16 * slots
+    args = _cache(17, lens, new, 1, Hq, Hkv, D)
+    a, la, ws = _check_attn(args)
+    assert int(_pieces(ws, slots, Hkv)[long_at].min()) >= 16
+    b, lb, _ = _check_attn(args)
+    assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+def test_short_sequences_stay_whole(dev):
+    lens = [(37 * b) % 250 for b in range(60)]
+    args = _cache(18, lens, [1] * 60, 1, 8, 2, 128)
+    _, _, ws = _check_attn(args)
+    assert int(_pieces(ws, 60, 2).max()) == 0
