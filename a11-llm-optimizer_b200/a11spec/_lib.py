@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liba11spec.so")
@@ -97,7 +98,7 @@ lib = _load()
 
 
 def _load_fast():
-    """a11spec._fast (cpp/fast_ops.cpp), built on the first import where it is missing."""
+    """a11spec._fast (cpp/fast_ops.cpp), built where it is missing."""
     import importlib
     if not os.path.exists(os.path.join(HERE, "_fast.so")):
         import importlib.util
@@ -112,7 +113,22 @@ def _load_fast():
     return mod
 
 
-fast = _load_fast()
+_fast_lock = threading.Lock()
+
+
+def __getattr__(name: str):
+    """`fast`, the layer operators' module: loaded when one of them is first called,
+    since it needs a compiler or a build for this torch and nothing else here does."""
+    if name != "fast":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    with _fast_lock:
+        if "fast" not in globals():
+            try:
+                globals()["fast"] = _load_fast()
+            except Exception as e:
+                raise ImportError("add_rms_norm, linear and chunk_attention need a11spec._fast, which could be neither "
+                                  f"loaded nor built: {e}") from e
+    return globals()["fast"]
 
 
 def check(rc: int) -> None:
