@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -38,12 +39,7 @@ class A11Error(RuntimeError):
 
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
-        import importlib.util
-        spec = importlib.util.spec_from_file_location(
-            "_a11spec_build", os.path.join(os.path.dirname(HERE), "build.py"))
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
-        mod.build()
+        _build_module().build()
     lib = C.CDLL(LIB_PATH)
     vp, i32, i64, f32, sz = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
     lib.a11s_abi_version.restype = C.c_int
@@ -97,19 +93,25 @@ def _load() -> C.CDLL:
 lib = _load()
 
 
+def _build_module():
+    """build.py, which lies beside this package."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("_a11spec_build", os.path.join(os.path.dirname(HERE), "build.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
 def _load_fast():
-    """a11spec._fast (cpp/fast_ops.cpp), built where it is missing."""
-    import importlib
-    if not os.path.exists(os.path.join(HERE, "_fast.so")):
-        import importlib.util
-        spec = importlib.util.spec_from_file_location(
-            "_a11spec_build", os.path.join(os.path.dirname(HERE), "build.py"))
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
-        mod.build_fast()
+    """a11spec._fast (cpp/fast_ops.cpp) of this interpreter, this torch and these sources, built where it is missing."""
+    import importlib.util
+    path = _build_module().build_fast()
     import torch  # noqa: F401  (its libraries first)
-    mod = importlib.import_module("a11spec._fast")
+    spec = importlib.util.spec_from_file_location("a11spec._fast", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
     mod.set_error_class(A11Error)
+    sys.modules["a11spec._fast"] = mod
     return mod
 
 

@@ -17,7 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT = os.path.join(HERE, "a11spec", "liba11spec.so")
 CPP = os.path.join(HERE, "cpp")
-FAST_OUT = os.path.join(HERE, "a11spec", "_fast.so")
+FAST_DIR = os.path.join(HERE, "a11spec")
+FAST_SOURCES = (os.path.join(CPP, "fast_ops.cpp"), os.path.join(INCLUDE, "a11spec.h"))
 VERIFIER_OUT = os.path.join(CPP, "libspec_verifier.so")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -80,15 +81,32 @@ def build_verifier(force: bool = False) -> str:
     return VERIFIER_OUT
 
 
-def build_fast(force: bool = False) -> str:
-    """a11spec/_fast.so: the layer operators' argument checks and calls in C++
-    (g++ against this interpreter's and this torch's headers)."""
-    src = os.path.join(CPP, "fast_ops.cpp")
-    hdr = os.path.join(INCLUDE, "a11spec.h")
-    if not force and os.path.exists(FAST_OUT) and all(
-            os.path.getmtime(p) <= os.path.getmtime(FAST_OUT) for p in (src, hdr)):
-        return FAST_OUT
+def fast_path() -> str:
+    """Where this interpreter's and this torch's a11spec._fast belongs: the name carries
+    what it is compiled against and its sources, so that no other build is taken for it."""
+    import hashlib
     import sysconfig
+
+    import torch
+    abi = "|".join((sysconfig.get_config_var("SOABI") or sys.version, torch.__version__, str(getattr(torch.version, "git_version", None)),
+                    str(torch._C._GLIBCXX_USE_CXX11_ABI)))
+    src = hashlib.sha256()
+    for p in FAST_SOURCES:
+        with open(p, "rb") as f:
+            src.update(f.read())
+    return os.path.join(FAST_DIR, f"_fast-{hashlib.sha256(abi.encode()).hexdigest()[:10]}-{src.hexdigest()[:10]}.so")
+
+
+def build_fast(force: bool = False) -> str:
+    """a11spec/_fast-*.so: the layer operators' argument checks and calls in C++
+    (g++ against this interpreter's and this torch's headers). Safe to call from
+    several processes at once: one builds, and the file appears when it is whole."""
+    out = fast_path()
+    if not force and os.path.exists(out):
+        return out
+    import fcntl
+    import sysconfig
+    import tempfile
 
     import torch
     root = os.path.dirname(torch.__file__)
@@ -98,13 +116,26 @@ def build_fast(force: bool = False) -> str:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for d in inc:
         cmd += ["-isystem" if d != INCLUDE else "-I", d]
-    cmd += ["-o", FAST_OUT + ".tmp", src, "-L", os.path.dirname(OUT), "-la11spec", "-Wl,-rpath,$ORIGIN", "-L", lib,
-            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{lib}"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
-    os.replace(FAST_OUT + ".tmp", FAST_OUT)
-    return FAST_OUT
+    lock = os.open(FAST_DIR, os.O_RDONLY)
+    try:
+        fcntl.flock(lock, fcntl.LOCK_EX)  # on the folder: leaves no file behind
+        if not force and os.path.exists(out):  # built by the one that held the lock
+            return out
+        with tempfile.TemporaryDirectory(prefix=".fast-", dir=FAST_DIR) as tmp:
+            made = os.path.join(tmp, "_fast.so")
+            r = subprocess.run(cmd + ["-o", made, FAST_SOURCES[0], "-L", os.path.dirname(OUT), "-la11spec",
+                                      "-Wl,-rpath,$ORIGIN", "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+                                      "-lc10_cuda", f"-Wl,-rpath,{lib}"], capture_output=True, text=True)
+            if r.returncode != 0:
+                raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
+            os.replace(made, out)
+        same_abi = out[:-len("-0123456789.so")]
+        for old in glob.glob(glob.escape(same_abi) + "-*.so"):  # of earlier sources
+            if old != out:
+                os.remove(old)
+    finally:
+        os.close(lock)
+    return out
 
 
 if __name__ == "__main__":

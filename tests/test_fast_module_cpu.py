@@ -8,7 +8,7 @@ PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 
 
 def _package_without_fast(tmp_path):
     """A copy of the package (links) that has neither a11spec._fast nor what builds it."""
-    os.makedirs(tmp_path / "a11spec")
+    os.makedirs(tmp_path / "a11spec", exist_ok=True)
     for f in sorted(os.listdir(os.path.join(PKG, "a11spec"))):
         if f.endswith(".py") or f == "liba11spec.so":
             os.symlink(os.path.join(PKG, "a11spec", f), tmp_path / "a11spec" / f)
@@ -53,3 +53,75 @@ else:
     raise SystemExit("no error")
 """, PKG)
     assert r.returncode == 0, r.stderr
+
+
+# --------------------------------------------------------------------------- the build
+def _tree_with_compiler(tmp_path):
+    """The package with its sources (links), no built module, and on PATH a g++ that takes
+    its time, logs its runs and puts out the module that the real one made."""
+    path = _package_without_fast(tmp_path / "pkg")
+    os.symlink(os.path.join(PKG, "build.py"), os.path.join(path, "build.py"))
+    os.symlink(os.path.join(PKG, "cpp"), os.path.join(path, "cpp"))
+    os.symlink(os.path.join(os.path.dirname(PKG), "include"), tmp_path / "include")
+    os.makedirs(tmp_path / "bin")
+    gxx = tmp_path / "bin" / "g++"
+    gxx.write_text("""#!/bin/sh
+echo run >> "$LOG"
+while [ "$1" != -o ]; do shift; done
+head -c 1000 "$MODULE" > "$2"
+sleep 2
+cat "$MODULE" > "$2"
+chmod +x "$2"
+""")
+    gxx.chmod(0o755)
+    import a11spec._lib as lib
+    env = dict(LOG=str(tmp_path / "log"), MODULE=sys.modules["a11spec._fast"].__file__ if lib.fast else "",
+               PATH=str(tmp_path / "bin") + os.pathsep + os.environ["PATH"], PYTHONPATH=path)
+    return path, env
+
+
+USE = "import torch, a11spec; from a11spec import _lib; assert _lib.fast.row_stride(torch.zeros(2, 8), 8) == 8"
+
+
+def test_a_module_of_another_build_is_not_loaded(tmp_path):
+    path, env = _tree_with_compiler(tmp_path)
+    for name in ("_fast.so", "_fast-0123456789-0123456789.so"):  # of another torch, or of other sources
+        with open(os.path.join(path, "a11spec", name), "wb") as f:
+            f.write(b"not this one")
+    for _ in range(2):
+        r = _python(USE, path, **{k: v for k, v in env.items() if k != "PYTHONPATH"})
+        assert r.returncode == 0, r.stderr
+    assert open(env["LOG"]).read() == "run\n"  # built once, found the second time
+
+
+def test_the_name_follows_torch_and_the_sources(tmp_path):
+    path, env = _tree_with_compiler(tmp_path)
+    r = _python("""
+import importlib.util, os, shutil, sys, torch
+spec = importlib.util.spec_from_file_location("b", os.path.join(os.environ["TREE"], "build.py"))
+b = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(b)
+names = [b.fast_path()]
+torch.__version__ += ".other"
+names.append(b.fast_path())
+copy = os.path.join(os.environ["TREE"], "changed.h")
+shutil.copy(b.FAST_SOURCES[1], copy)
+with open(copy, "a") as f:
+    f.write("/* */")
+b.FAST_SOURCES = (b.FAST_SOURCES[0], copy)
+names.append(b.fast_path())
+assert len(set(names)) == 3, names
+""", path, TREE=path)
+    assert r.returncode == 0, r.stderr
+
+
+def test_processes_that_build_at_once(tmp_path):
+    path, env = _tree_with_compiler(tmp_path)
+    ranks = [subprocess.Popen([sys.executable, "-c", USE], env={**os.environ, **env}, stderr=subprocess.PIPE, text=True)
+             for _ in range(3)]
+    for r in ranks:
+        err = r.communicate(timeout=300)[1]
+        assert r.returncode == 0, err
+    assert open(env["LOG"]).read() == "run\n"
+    left = [f for f in os.listdir(os.path.join(path, "a11spec")) if "fast" in f]
+    assert len(left) == 1, left
