@@ -7,6 +7,7 @@
 // documented in a11spec/ops.py; the kernels are those of the C ABI
 // (include/a11spec.h).
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -14,6 +15,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
+#include <exception>
 #include <sstream>
 #include <string>
 
@@ -124,8 +126,8 @@ PyObject *guarded(F f) {
         } else if (!PyErr_Occurred()) {
             PyErr_SetString(PyExc_RuntimeError, r.message.c_str());
         }
-    } catch (const std::exception &e) {
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {  // torch's own keep their types: an allocation that fails is torch.OutOfMemoryError
+        if (!PyErr_Occurred()) torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }

@@ -76,3 +76,22 @@ def test_short_sequences_stay_whole(dev):
     args = _cache(18, lens, [1] * 60, 1, 8, 2, 128)
     _, _, ws = _check_attn(args)
     assert int(_pieces(ws, 60, 2).max()) == 0
+
+
+# --------------------------------------------------------------------------- errors
+def test_failed_allocation_is_torchs_error(dev):
+    """An output that does not fit raises torch.OutOfMemoryError, as callers that shrink
+    their batch expect, and the next call works. The limit is this process's own."""
+    x, w = torch.ones(200000, 8, dtype=BF, device=dev), torch.ones(4096, 8, dtype=BF, device=dev)  # 1.6 GB of output
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            a11spec.linear(x, w)
+        y = a11spec.linear(x[:1000], w)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert bool((y == 8).all())
+    assert a11spec.linear(x, w).shape == (200000, 4096)
