@@ -260,7 +260,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise A11Error(_lib.EINVAL, f"linear: activation {activation!r}, not None, 'silu' or 'gelu'")
-    if ws is None and check_status:
+    if ws is None and check_status and isinstance(x, torch.Tensor):
         ws = workspace(256, x.device)
     out = _lib.fast.linear(x, weight, bias, act, gate, gate_bias, residual, x_scale, weight_scale, gate_scale, out, ws)
     if check_status:
