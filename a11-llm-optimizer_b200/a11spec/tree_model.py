@@ -181,9 +181,9 @@ class TreeDecoder:
         self.k_pool[layer, page, off] = k[b, i].to(torch.bfloat16)
         self.v_pool[layer, page, off] = v[b, i].to(torch.bfloat16)
 
-    def _forward(self, tokens, parents, n_nodes, page_table, ctx_lens, positions, max_kv_len=None):
-        """Logits of every token. With max_kv_len the tokens are a chunk (each
-        follows the one before it), else a tree of `parents`."""
+    def _forward(self, tokens, parents, n_nodes, page_table, ctx_lens, positions, max_kv_len=None, head=True):
+        """Logits of every token (None without the head). With max_kv_len the tokens
+        are a chunk (each follows the one before it), else a tree of `parents`."""
         B, N = tokens.shape
         ar = torch.arange(N, device=tokens.device)
         live = ar.unsqueeze(0) < n_nodes.unsqueeze(1)
@@ -201,7 +201,7 @@ class TreeDecoder:
         h = self.w["token_embd.weight"][tokens.clamp_min(0).long()]  # [B, N, n_embd]
         hn = self._layers_fused(h, attend) if self.fused else self._layers(h, attend)
         self.forwards += 1
-        return self._head(hn)
+        return self._head(hn) if head else None
 
     def _layers(self, h, attend):
         cfg = self.cfg
@@ -269,7 +269,8 @@ class TreeDecoder:
         """K/V of the prompt tokens [B, T] at positions 0 .. T-1, in chunks of up
         to `chunk` tokens (each attends to the earlier chunks and to its own
         prefix): chain trees up to 64, a11s_chunk_attention beyond. Returns the
-        logits of the last chunk."""
+        logits of the last chunk; the others' are not computed (a vocabulary wide,
+        they would outweigh a long chunk's layers and cache)."""
         B, T = tokens.shape
         logits = None
         for c0 in range(0, T, chunk):
@@ -279,7 +280,7 @@ class TreeDecoder:
             ctx = torch.full((B,), c0, dtype=torch.int32, device=tokens.device)
             pos = c0 + torch.arange(n, device=tokens.device).unsqueeze(0).expand(B, n)
             logits = self._forward(tokens[:, c0:c0 + n].contiguous(), par, nn, page_table, ctx, pos,
-                                   max_kv_len=c0 + n if chunk > 64 else None)
+                                   max_kv_len=c0 + n if chunk > 64 else None, head=c0 + n == T)
         return logits
 
 
