@@ -24,7 +24,8 @@ The target model is any object with:
   [num_layers, pages, 16, Hkv, D] with a ``num_layers`` attribute: the paged KV
   cache the model's attention reads, one slab per layer);
 * ``prefill(tokens, page_table, ctx_lens)``: write the K/V of tokens
-  [B, T] at positions 0 .. T-1 (ctx_lens is 0 on entry; the caller sets it);
+  [B, T] at positions 0 .. T-1 (ctx_lens is 0 on entry; the caller sets it),
+  with a `chunk` argument where the stream is asked for a prefill_chunk;
 * ``forward_tree(tokens, parents, n_nodes, page_table, ctx_lens)`` ->
   logits [B, N, V] (bf16 or fp32): node i's row judges its children.
 """
@@ -40,14 +41,17 @@ from .decoder import SpeculativeDecoder
 
 def speculative_stream(model, prompts: torch.Tensor, max_new_tokens: int, decoder: SpeculativeDecoder,
                        pages: ops.KVPagePool, max_pages: int, learn: bool = True,
-                       uniforms_fn=None) -> Iterator[List[List[int]]]:
+                       uniforms_fn=None, prefill_chunk: Optional[int] = None) -> Iterator[List[List[int]]]:
     """Yield, per target forward, the committed tokens of every sequence
     (a list per sequence, empty once it has max_new_tokens). prompts: int32
     [B, T], T >= 2, on the model's device. Page tables and lengths live on
     the device; the loop reads
     back only the committed tokens it yields. The decoder's temperature
     decides the rule: None = greedy, else one-hot sampling at that temperature
-    (uniforms from `uniforms_fn(B, N)` or the decoder's own generator)."""
+    (uniforms from `uniforms_fn(B, N)` or the decoder's own generator).
+    prefill_chunk: passed on as model.prefill(..., chunk=prefill_chunk) (a
+    TreeDecoder takes prompts in chunks above 64 through a11s_chunk_attention);
+    None leaves the model's default."""
     dev = prompts.device
     B, T = prompts.shape
     if T < 2:
@@ -57,7 +61,8 @@ def speculative_stream(model, prompts: torch.Tensor, max_new_tokens: int, decode
     ctx_lens = torch.zeros(B, dtype=torch.int32, device=dev)
     # the prompt's last token is the first tree's root: prefill the others
     pages.reserve(page_table, ctx_lens, torch.full((B,), T - 1, dtype=torch.int32, device=dev), check_status=True)
-    model.prefill(prompts[:, :T - 1].contiguous(), page_table, ctx_lens)
+    how = {} if prefill_chunk is None else {"chunk": prefill_chunk}
+    model.prefill(prompts[:, :T - 1].contiguous(), page_table, ctx_lens, **how)
     last = prompts[:, T - 2:].contiguous().to(torch.int32)
     grown = torch.empty_like(ctx_lens)
     hist_buf = (torch.empty(B, N + 3, dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int32, device=dev))

@@ -3,6 +3,9 @@ logits do not depend on how the prompt is cut (beyond the roundings)."""
 import pytest
 import torch
 
+from a11spec import ops
+from a11spec.decoder import SpeculativeDecoder
+from a11spec.generate import speculative_stream
 from a11spec.ops import KVPagePool
 from a11spec.tree_model import TreeDecoder, synthetic_tensors
 from test_tree_decoder_gpu import CFG, GOLD, PAGES, TOL_REL
@@ -69,3 +72,24 @@ def test_cache_and_logits_do_not_depend_on_the_chunks(dev, fused, chunk):
     n = min(la.shape[1], lb.shape[1])
     x, y = la[:, -n:].double(), lb[:, -n:].double()
     assert float(((x - y).abs().amax(2) / x.abs().amax(2)).max()) <= 2 * TOL_REL
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_stream_prefills_in_long_chunks(dev, fused, monkeypatch):
+    """speculative_stream(prefill_chunk=...) takes the prompt through chunk attention and
+    commits the tokens that the default commits, up to the first step where the reference's
+    own top two logits are closer than a rounding."""
+    calls = []
+    attend = ops.chunk_attention
+    monkeypatch.setattr(ops, "chunk_attention", lambda q, *a, **k: calls.append(q.shape[1]) or attend(q, *a, **k))
+    model = TreeDecoder(synthetic_tensors(CFG, int(GOLD["weight_seed"])), CFG, PAGES, dev, fused=fused)
+    dec = SpeculativeDecoder(table=torch.zeros((1 << 10, 4, 2), dtype=torch.int32), log2_buckets=10, width_root=2, width_inner=1,
+                             max_depth=5, max_nodes=16, temperature=None, device=dev)
+    prompt = torch.from_numpy(GOLD["prompt"]).to(dev).view(1, -1).contiguous()
+    out = []
+    for new in speculative_stream(model, prompt, 24, dec, KVPagePool(PAGES, dev), max_pages=16, learn=True, prefill_chunk=512):
+        out += new[0]
+    assert calls == [prompt.shape[1] - 1] * CFG.n_layers
+    first_close = int((GOLD["gaps"] < 0.1).argmax()) if (GOLD["gaps"] < 0.1).any() else 24
+    n = min(first_close, 20)
+    assert out[:n] == GOLD["tokens"].tolist()[:n]
