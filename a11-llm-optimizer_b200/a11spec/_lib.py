@@ -75,6 +75,7 @@ def _load() -> C.CDLL:
     lib.a11s_add_rms_norm.argtypes = [i32, vp, i64, vp, i64, vp, i32, i32, f32, vp, i64, i32, vp, i64, vp, vp]
     lib.a11s_linear.argtypes = [i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, i64, vp, i64,
                                 vp, sz, vp]
+    lib.a11s_linear_plan.argtypes = [i32, i32, i32, i32, i32, C.POINTER(i32), C.POINTER(i32)]
     lib.a11s_chunk_attention_workspace_bytes.restype = sz
     lib.a11s_chunk_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32]
     lib.a11s_chunk_attention.argtypes = [vp, i64, vp, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, f32,
@@ -83,7 +84,7 @@ def _load() -> C.CDLL:
                  "a11s_ngram_expand", "a11s_verify_chain", "a11s_accept_static", "a11s_kv_pool_init",
                  "a11s_kv_reserve", "a11s_kv_release", "a11s_kv_free_sequences", "a11s_ngram_update",
                  "a11s_next_roots", "a11s_lm_head", "a11s_accept_recorded", "a11s_add_rms_norm", "a11s_linear",
-                 "a11s_chunk_attention"):
+                 "a11s_linear_plan", "a11s_chunk_attention"):
         getattr(lib, name).restype = C.c_int
     if lib.a11s_abi_version() != 1:
         raise ImportError("liba11spec.so ABI version mismatch")
@@ -146,4 +147,5 @@ def symbols():
             "a11s_ngram_expand", "a11s_ngram_bucket", "a11s_verify_chain", "a11s_kv_pool_init",
             "a11s_kv_reserve", "a11s_kv_release", "a11s_kv_free_sequences", "a11s_ngram_update",
             "a11s_next_roots", "a11s_lm_head_keys_bytes", "a11s_lm_head", "a11s_accept_recorded",
-            "a11s_add_rms_norm", "a11s_linear", "a11s_chunk_attention_workspace_bytes", "a11s_chunk_attention"]
+            "a11s_add_rms_norm", "a11s_linear", "a11s_linear_plan", "a11s_chunk_attention_workspace_bytes",
+            "a11s_chunk_attention"]

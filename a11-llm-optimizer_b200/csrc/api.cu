@@ -778,4 +778,21 @@ int a11s_linear(int32_t dtype, const void *x, int64_t x_stride, const float *x_s
     return A11S_OK;
 }
 
+int a11s_linear_plan(int32_t dtype, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t gated, int32_t *tile, int32_t *split) {
+    if (dtype != A11S_BF16 && dtype != A11S_E4M3) return fail(A11S_EINVAL, "a11s_linear_plan: dtype %d", dtype);
+    if (rows < 1 || in_dim < 1 || out_dim < 1 || rows > A11S_LINEAR_MAX || out_dim > A11S_LINEAR_MAX || in_dim > A11S_LINEAR_MAX / 2)
+        return fail(A11S_EINVAL, "a11s_linear_plan: bad sizes");
+    if (!tile || !split) return fail(A11S_EINVAL, "a11s_linear_plan: null required pointer");
+    a11s::LinearArgs a{};
+    a.rows = rows;
+    a.K = in_dim;
+    a.N = out_dim;
+    a.e4m3 = dtype == A11S_E4M3;
+    a.gate = gated ? tile : nullptr;  // only asked whether there is one
+    const a11s::LinearPlan plan = a11s::linear_plan(a);
+    *tile = plan.tile;
+    *split = plan.split;
+    return A11S_OK;
+}
+
 }  // extern "C"

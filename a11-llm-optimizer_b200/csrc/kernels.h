@@ -245,6 +245,10 @@ struct LinearArgs {
     StatusWord *status;           // nullable
 };
 cudaError_t launch_linear(const LinearArgs &a, cudaStream_t s);
+struct LinearPlan {
+    int32_t tile, split;  // a11s_linear_plan
+};
+LinearPlan linear_plan(const LinearArgs &a);  // of a's sizes, type and gate
 // rows at most kSkinnyRows: the weight-streaming kernel
 constexpr int kSkinnyRows = 32;
 cudaError_t launch_linear_skinny(const LinearArgs &a, cudaStream_t s);

@@ -698,7 +698,7 @@ int tile_slots(int split, int sms) {
 // For instance 64 x 8192 -> 2048: 64/4 14.2 us, 32/2 18.7, 64/1 33.6, pairs 43.9;
 // 768 x 4096 -> 4096: pairs 26.3, 128/2 45.5; 197 x 1000 -> 1531: 64/2 10.0, 32/1 10.4.
 struct Plan {
-    int bn = 0, split = 1;  // bn 0: linear_pair
+    int bn = kPairN, split = 1;
 };
 Plan choose(const LinearArgs &a, int slices, int sms) {
     const auto tiles = [&](int m, int n) { return (long long)((a.rows + m - 1) / m) * ((a.N + n - 1) / n); };
@@ -720,6 +720,11 @@ Plan choose(const LinearArgs &a, int slices, int sms) {
             }
         }
     return best;
+}
+
+int k_slices(const LinearArgs &a) {
+    const int elems = a.e4m3 ? kSliceBytes : kSliceBytes / 2;
+    return (a.K + elems - 1) / elems;
 }
 
 template <bool E4M3, bool GATED, int BN>
@@ -804,18 +809,23 @@ cudaError_t launch_type(const LinearArgs &a, cudaStream_t s) {
     p.N = a.N;
     p.act = a.act;
     p.status = a.status;
-    const int elems = E4M3 ? kSliceBytes : kSliceBytes / 2;
-    p.slices = (a.K + elems - 1) / elems;
+    p.slices = k_slices(a);
     const int sms = device_sms();
     const Plan plan = choose(a, p.slices, sms);
-    if (plan.bn == 0) return launch_pair<E4M3, GATED>(a, p, sms, s);
     switch (plan.bn) {
+        case kPairN: return launch_pair<E4M3, GATED>(a, p, sms, s);
         case 32: return launch_tile<E4M3, GATED, 32>(a, p, plan.split, s);
         case 64: return launch_tile<E4M3, GATED, 64>(a, p, plan.split, s);
         default: return launch_tile<E4M3, GATED, 128>(a, p, plan.split, s);
     }
 }
 }  // namespace
+
+LinearPlan linear_plan(const LinearArgs &a) {
+    if (a.rows <= kSkinnyRows) return {0, 1};
+    const Plan plan = choose(a, k_slices(a), device_sms());
+    return {plan.bn, plan.split};
+}
 
 cudaError_t launch_linear(const LinearArgs &a, cudaStream_t s) {
     if (a.rows <= kSkinnyRows) return launch_linear_skinny(a, s);

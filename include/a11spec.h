@@ -358,6 +358,13 @@ int a11s_linear(int32_t dtype, const void *x, int64_t x_stride, const float *x_s
                 const void *residual, int64_t residual_stride, void *out, int64_t out_stride,
                 void *workspace, size_t workspace_bytes, void *stream);
 
+/* Which kernel a11s_linear takes for a size on the current device, for timing and
+ * tests: *tile 0 (up to 32 rows, the weights streamed), 32, 64 or 128 (weight rows
+ * of a tile with 128 rows of x; *split CTAs share in_dim) or 256 (CTA pairs). gated:
+ * with a gate. */
+int a11s_linear_plan(int32_t dtype, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t gated,
+                     int32_t *tile, int32_t *split);
+
 /* ------------------------------------------------------------------------ K4
  * In-place compaction of the accepted path. Replaces the host block-table
  * bookkeeping of PagedKVCacheManager::append_token / free_sequence
