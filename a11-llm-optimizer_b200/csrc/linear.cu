@@ -106,13 +106,11 @@ template <int THREADS>
 __device__ __forceinline__ void epilogue_barrier() {
     asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
-// A warp's 32 rows of C consecutive outputs from shared memory (rows C + 1
-// floats apart): the residual is added and the row segments written coalesced.
-template <int C>
+// A warp's 32 rows of 16 consecutive outputs from shared memory (rows 17 floats
+// apart), two rows an access: the residual is added and the row segments written.
 __device__ __forceinline__ void write_rows(const float *stage, const LinParams &p, int m0, int n0, int lane) {
-    constexpr int kRows = C >= 32 ? 1 : 32 / C, kParts = C >= 32 ? C / 32 : 1;  // rows per access, accesses per row
-    constexpr int kSteps = 32 / kRows * kParts, kBatch = kSteps < 8 ? kSteps : kSteps <= 16 ? 8 : 16;
-    const int r0 = C >= 32 ? 0 : lane / C, c0 = C >= 32 ? lane : lane % C;
+    constexpr int kSteps = 16, kBatch = 8;
+    const int r0 = lane >> 4, c = lane & 15;
 #pragma unroll 1
     for (int i0 = 0; i0 < kSteps; i0 += kBatch) {
         // all of a batch's residual loads (absent elements: the last one again) before
@@ -120,18 +118,16 @@ __device__ __forceinline__ void write_rows(const float *stage, const LinParams &
         __nv_bfloat16 res[kBatch];
         if (p.residual) {
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int r = (i0 + i) / kParts * kRows + r0, c = c0 + (i0 + i) % kParts * 32;
-                res[i] = p.residual[(int64_t)min(m0 + r, p.rows - 1) * p.res_stride + min(n0 + c, p.N - 1)];
-            }
+            for (int i = 0; i < kBatch; ++i)
+                res[i] = p.residual[(int64_t)min(m0 + 2 * (i0 + i) + r0, p.rows - 1) * p.res_stride + min(n0 + c, p.N - 1)];
         } else {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) res[i] = __float2bfloat16_rn(0.0f);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int r = (i0 + i) / kParts * kRows + r0, c = c0 + (i0 + i) % kParts * 32;
-            const float y = stage[r * (C + 1) + c] + __bfloat162float(res[i]);
+            const int r = 2 * (i0 + i) + r0;
+            const float y = stage[r * 17 + c] + __bfloat162float(res[i]);
             if (m0 + r < p.rows && n0 + c < p.N) p.out[(int64_t)(m0 + r) * p.out_stride + n0 + c] = __float2bfloat16_rn(y);
         }
     }
@@ -600,7 +596,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) st[lane * 17 + e] = v[e0 + e];
                         __syncwarp();
-                        write_rows<16>(st, p, mw, n + e0, lane);
+                        write_rows(st, p, mw, n + e0, lane);
                         __syncwarp();
                     }
                 }
