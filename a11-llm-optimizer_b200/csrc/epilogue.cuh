@@ -5,6 +5,7 @@
 
 namespace a11s {
 
+// Below v = -87.3 the denominator passes 2^126 and the quotient is 0 (of y above -2^-119).
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 // v Phi(v) with Phi(-|v|) = exp(-v^2 / 2) erfcx(|v| / sqrt(2)) / 2, where erfcx(z) =
 // exp(z^2) erfc(z) is a polynomial in t = 1 / (1 + 0.38 z) (the form of Hastings'
