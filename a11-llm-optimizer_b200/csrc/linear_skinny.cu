@@ -184,13 +184,14 @@ __global__ void __launch_bounds__(512) linear_skinny_kernel(const SkinnyParams p
 template <bool E4M3, bool GATED, int NT, bool WIDE>
 cudaError_t launch_nt(const SkinnyParams &p, cudaStream_t s) {
     // Two column tiles a block where that still gives every SM a block and pays:
-    // for a gated product of few rows, gate and weight rows then come in longer runs
-    // (1 x 2048 -> 8192: 13.1 us against 14.2); for more rows x is read half as
-    // often (17 x 2048 -> 5120 e4m3: 7.4 against 8.6; bf16 9.5 against 10.8). Not
-    // for bf16 products of up to 16 rows (9 x 2048 -> 5120: 7.9 against 6.9), gated
-    // ones of more (32 rows: 32 against 20, registers) and e4m3 of over 24 (32 x 2048
-    // -> 5120: 8.7 against 7.4).
-    constexpr bool kTwo = GATED ? NT <= 2 : E4M3 ? NT == 2 || NT == 3 : NT >= 3;
+    // for a gated product of few rows, gate and weight rows then come in longer runs,
+    // and at the rows below x is read half as often; else the registers that a second
+    // tile takes cost more. One tile / two, us: gated 2048 -> 8192, bf16 1 row 14.5 / 12.6,
+    // 16 rows 16.3 / 15.0, 17 rows 17.7 / 20.3; e4m3 8 rows 9.8 / 8.8, 16 rows 11.1 / 12.5
+    // (spills); 2048 -> 5120, bf16 16 rows 6.9 / 8.3, 17 rows 7.2 / 8.9, 25 rows 11.6 /
+    // 10.2; e4m3 16 rows 5.3 / 6.1, 17 rows 8.4 / 7.0, 25 rows 8.9 / 9.5. The same side
+    // won at K from 1024 to 8192 and N from 5120 to 16384.
+    constexpr bool kTwo = GATED ? NT <= (E4M3 ? 1 : 2) : NT == (E4M3 ? 3 : 4);
     const int mt = kTwo && p.N >= 32 * 148 ? 2 : 1;
     const int blocks = (p.N + 16 * mt - 1) / (16 * mt);
     // 8 warps share K; 16 when the blocks do not fill the SMs and K has slices for

@@ -61,3 +61,23 @@ def test_every_tiling_is_among_them():
     want = {(g, t, s) for g in (False, True) for t in (32, 64, 128) for s in (1, 2, 4, 8)} - {(True, 32, 8)}
     want |= {(g, t, 1) for g in (False, True) for t in (0, 256)}
     assert {p[:3] for p in PLANS} == want
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 24, 25, 32])
+@pytest.mark.parametrize("K,N", [(2112, 4741), (272, 5000), (288, 4735), (4112, 83), (1040, 2048)])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("gated", [False, True])
+def test_streamed_weights(dev, rows, K, N, e4m3, gated):
+    """Every number of row tiles, one and two column tiles a block (N from 32 * 148 on), 8 and
+    16 warps (few blocks over a long K), rows in whole 32-byte pieces and not, and the largest
+    exchange of sums."""
+    activation, bias, residual = ("silu", True, True) if gated else ("gelu", True, True)
+    assert _plan(e4m3, rows, K, N, gated) == (0, 1)
+    x, w, kw = _linear_case(rows + 7 * K + 31 * N, rows, K, N, e4m3, gated, bias, residual)
+    ref, tol = _linear_ref(x, w, kw, activation)
+    buf = torch.full((rows + 2, N), math.nan, dtype=BF, device="cuda")
+    y = a11spec.linear(x, w, activation=activation, out=buf[1:-1], check_status=True, **kw)
+    r = R.worst(y, ref, tol)
+    assert r <= 1, r
+    assert bool(buf[0].isnan().all()) and bool(buf[-1].isnan().all())
+    assert torch.equal(y, a11spec.linear(x, w, activation=activation, **kw))
