@@ -37,6 +37,15 @@ class A11Error(RuntimeError):
         self.code = code
 
 
+def _build_module():
+    """build.py, which lies beside this package."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("_a11spec_build", os.path.join(os.path.dirname(HERE), "build.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         _build_module().build()
@@ -92,15 +101,6 @@ def _load() -> C.CDLL:
 
 
 lib = _load()
-
-
-def _build_module():
-    """build.py, which lies beside this package."""
-    import importlib.util
-    spec = importlib.util.spec_from_file_location("_a11spec_build", os.path.join(os.path.dirname(HERE), "build.py"))
-    mod = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(mod)
-    return mod
 
 
 def _load_fast():

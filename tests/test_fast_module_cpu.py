@@ -125,3 +125,14 @@ def test_processes_that_build_at_once(tmp_path):
     assert open(env["LOG"]).read() == "run\n"
     left = [f for f in os.listdir(os.path.join(path, "a11spec")) if "fast" in f]
     assert len(left) == 1, left
+
+
+def test_missing_library_is_built_on_import(tmp_path):
+    path, env = _tree_with_compiler(tmp_path)
+    os.symlink(os.path.join(PKG, "csrc"), os.path.join(path, "csrc"))
+    lib = os.path.join(path, "a11spec", "liba11spec.so")
+    env.update(MODULE=os.path.realpath(lib), NVCC=str(tmp_path / "bin" / "g++"))
+    os.unlink(lib)
+    r = _python("import a11spec; a11spec.ngram_bucket(1, 2, 10)", path, **{k: v for k, v in env.items() if k != "PYTHONPATH"})
+    assert r.returncode == 0, r.stderr
+    assert open(env["LOG"]).read() == "run\n"
