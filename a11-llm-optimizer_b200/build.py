@@ -7,10 +7,13 @@ it travels with the repository snapshot and is what the package loads.
 from __future__ import annotations
 
 import argparse
+import contextlib
+import fcntl
 import glob
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -32,6 +35,19 @@ NVCC_FLAGS = [
 ]
 
 
+@contextlib.contextmanager
+def building(folder: str):
+    """One process at a time builds into `folder`: under a lock on it (which leaves no
+    file behind), with a scratch folder from which the result moves to its place whole."""
+    lock = os.open(folder, os.O_RDONLY)
+    try:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        with tempfile.TemporaryDirectory(prefix=".build-", dir=folder) as tmp:
+            yield tmp
+    finally:
+        os.close(lock)
+
+
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
 
@@ -51,16 +67,20 @@ def up_to_date() -> bool:
 def build(force: bool = False, verbose: bool = False, extra=()) -> str:
     if not force and up_to_date():
         return OUT
-    cmd = [NVCC, *NVCC_FLAGS, *extra, "-I", INCLUDE, "-o", OUT + ".tmp", *sources()]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), file=sys.stderr)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
-    if verbose:
-        print(r.stdout + r.stderr, file=sys.stderr)
-    os.replace(OUT + ".tmp", OUT)
+    with building(os.path.dirname(OUT)) as tmp:
+        if not force and up_to_date():  # built by the one that held the lock
+            return OUT
+        made = os.path.join(tmp, "liba11spec.so")
+        cmd = [NVCC, *NVCC_FLAGS, *extra, "-I", INCLUDE, "-o", made, *sources()]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+            print(" ".join(cmd), file=sys.stderr)
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
+        if verbose:
+            print(r.stdout + r.stderr, file=sys.stderr)
+        os.replace(made, OUT)
     return OUT
 
 
@@ -104,9 +124,7 @@ def build_fast(force: bool = False) -> str:
     out = fast_path()
     if not force and os.path.exists(out):
         return out
-    import fcntl
     import sysconfig
-    import tempfile
 
     import torch
     root = os.path.dirname(torch.__file__)
@@ -116,25 +134,20 @@ def build_fast(force: bool = False) -> str:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for d in inc:
         cmd += ["-isystem" if d != INCLUDE else "-I", d]
-    lock = os.open(FAST_DIR, os.O_RDONLY)
-    try:
-        fcntl.flock(lock, fcntl.LOCK_EX)  # on the folder: leaves no file behind
+    with building(FAST_DIR) as tmp:
         if not force and os.path.exists(out):  # built by the one that held the lock
             return out
-        with tempfile.TemporaryDirectory(prefix=".fast-", dir=FAST_DIR) as tmp:
-            made = os.path.join(tmp, "_fast.so")
-            r = subprocess.run(cmd + ["-o", made, FAST_SOURCES[0], "-L", os.path.dirname(OUT), "-la11spec",
-                                      "-Wl,-rpath,$ORIGIN", "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
-                                      "-lc10_cuda", f"-Wl,-rpath,{lib}"], capture_output=True, text=True)
-            if r.returncode != 0:
-                raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
-            os.replace(made, out)
+        made = os.path.join(tmp, "_fast.so")
+        r = subprocess.run(cmd + ["-o", made, FAST_SOURCES[0], "-L", os.path.dirname(OUT), "-la11spec", "-Wl,-rpath,$ORIGIN",
+                                  "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+                                  f"-Wl,-rpath,{lib}"], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
+        os.replace(made, out)
         same_abi = out[:-len("-0123456789.so")]
         for old in glob.glob(glob.escape(same_abi) + "-*.so"):  # of earlier sources
             if old != out:
                 os.remove(old)
-    finally:
-        os.close(lock)
     return out
 
 

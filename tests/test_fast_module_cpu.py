@@ -136,3 +136,19 @@ def test_missing_library_is_built_on_import(tmp_path):
     r = _python("import a11spec; a11spec.ngram_bucket(1, 2, 10)", path, **{k: v for k, v in env.items() if k != "PYTHONPATH"})
     assert r.returncode == 0, r.stderr
     assert open(env["LOG"]).read() == "run\n"
+
+
+def test_processes_that_build_the_library_at_once(tmp_path):
+    """The same for liba11spec.so, which the import builds where it is missing."""
+    path, env = _tree_with_compiler(tmp_path)
+    os.symlink(os.path.join(PKG, "csrc"), os.path.join(path, "csrc"))
+    lib = os.path.join(path, "a11spec", "liba11spec.so")
+    env.update(MODULE=os.path.realpath(lib), NVCC=str(tmp_path / "bin" / "g++"))
+    os.unlink(lib)
+    ranks = [subprocess.Popen([sys.executable, "-c", "import a11spec; a11spec.ngram_bucket(1, 2, 10)"], env={**os.environ, **env},
+                              stderr=subprocess.PIPE, text=True) for _ in range(3)]
+    for r in ranks:
+        err = r.communicate(timeout=300)[1]
+        assert r.returncode == 0, err
+    assert open(env["LOG"]).read() == "run\n"
+    assert [f for f in os.listdir(os.path.join(path, "a11spec")) if f.startswith((".", "liba11"))] == ["liba11spec.so"]
