@@ -112,7 +112,10 @@ class TreeDecoder:
     tensors: name -> tensor with the reference's GGUF names; converted to the
     compute dtype on `device`. The K/V pools are [n_layers, num_pages, 16,
     n_head_kv, head_dim] bf16, the layout a11s_kv_compact moves (num_layers
-    slabs) and a11s_tree_attention reads one layer of."""
+    slabs) and a11s_tree_attention reads one layer of. Trees of several nodes need
+    the heads that a11s_tree_attention takes (head_dim 128, n_head = 8 n_head_kv);
+    models with other heads that a11s_chunk_attention takes prefill and decode one
+    token at a time through that."""
 
     def __init__(self, tensors: Dict[str, torch.Tensor], cfg: DecoderConfig, num_pages: int, device="cuda",
                  compute_dtype: torch.dtype = torch.bfloat16, fused=False):
@@ -132,6 +135,7 @@ class TreeDecoder:
         self.w = {k: v.to(self.device, compute_dtype).contiguous() for k, v in tensors.items()}
         self.num_layers = cfg.n_layers
         self.vocab = cfg.vocab
+        self.tree_heads = cfg.head_dim == 128 and cfg.n_head == 8 * cfg.n_head_kv
         shape = (cfg.n_layers, num_pages, PAGE_TOKENS, cfg.n_head_kv, cfg.head_dim)
         self.k_pool = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
         self.v_pool = torch.zeros_like(self.k_pool)
@@ -263,14 +267,18 @@ class TreeDecoder:
     def forward_tree(self, tokens, parents, n_nodes, page_table, ctx_lens) -> torch.Tensor:
         """Logits [B, N, V] of every node; node i's K/V land at slot ctx + i."""
         pos = ctx_lens.long().unsqueeze(1) + tree_depths(parents, n_nodes)
-        return self._forward(tokens, parents, n_nodes, page_table, ctx_lens, pos).contiguous()
+        # a tree of one node is a chunk of one token
+        chunk = tokens.shape[1] == 1 and not self.tree_heads
+        return self._forward(tokens, parents, n_nodes, page_table, ctx_lens, pos,
+                             max_kv_len=page_table.shape[1] * PAGE_TOKENS if chunk else None).contiguous()
 
     def prefill(self, tokens, page_table, ctx_lens=None, chunk: int = 64) -> Optional[torch.Tensor]:
         """K/V of the prompt tokens [B, T] at positions 0 .. T-1, in chunks of up
         to `chunk` tokens (each attends to the earlier chunks and to its own
-        prefix): chain trees up to 64, a11s_chunk_attention beyond. Returns the
-        logits of the last chunk; the others' are not computed (a vocabulary wide,
-        they would outweigh a long chunk's layers and cache)."""
+        prefix): chain trees up to 64, a11s_chunk_attention beyond and for heads
+        that trees do not take. Returns the logits of the last chunk; the others'
+        are not computed (a vocabulary wide, they would outweigh a long chunk's
+        layers and cache)."""
         B, T = tokens.shape
         logits = None
         for c0 in range(0, T, chunk):
@@ -280,7 +288,7 @@ class TreeDecoder:
             ctx = torch.full((B,), c0, dtype=torch.int32, device=tokens.device)
             pos = c0 + torch.arange(n, device=tokens.device).unsqueeze(0).expand(B, n)
             logits = self._forward(tokens[:, c0:c0 + n].contiguous(), par, nn, page_table, ctx, pos,
-                                   max_kv_len=c0 + n if chunk > 64 else None, head=c0 + n == T)
+                                   max_kv_len=c0 + n if chunk > 64 or not self.tree_heads else None, head=c0 + n == T)
         return logits
 
 
