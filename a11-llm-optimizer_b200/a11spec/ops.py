@@ -284,7 +284,9 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     K/V already sit in the pools [P, 16, Hkv, D] at positions ctx_lens[b] + i of
     page_table [B, maxpages]. Token i < n_new[b] (default n) sees positions
     0 .. ctx_lens[b] + i; the other rows come back as zeros. max_kv_len: an upper
-    bound of ctx_lens[b] + n_new[b] (default: what the page table holds).
+    bound of ctx_lens[b] + n_new[b] (default: what the page table holds). fp32 but
+    for the probabilities, which are bf16 in the product with V; a non-finite V row
+    of a live token may reach earlier tokens of its 128-key block.
     Returns (out, lse, ws); lse [B, n, Hq] fp32 with want_lse, else None; out
     overlaps no input. Pass ws
     again to reuse it; calls that overlap on the GPU need one each."""

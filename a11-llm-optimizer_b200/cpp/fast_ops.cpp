@@ -3,7 +3,8 @@
 //
 // One decoded token calls each of them several times per layer, and the kernels
 // take 2 to 8 us: checked in Python and called through ctypes a call takes 8 to
-// 13 us on the host, from here 4 to 6. Semantics, arguments and errors are
+// 13 us on the host, from here 3 to 5 with the outputs given and 4 to 8 where it
+// makes them. Semantics, arguments and errors are
 // documented in a11spec/ops.py; the kernels are those of the C ABI
 // (include/a11spec.h).
 #include <torch/csrc/Dtype.h>

@@ -39,6 +39,7 @@
 // complete. Measured slower: polling them ahead of time (941 us), one tile per CTA
 // with two CTAs per SM at D = 64 (55 us), a quarter of the exponentials as a
 // polynomial on the FMA units (983 us), two threads a row (1785 us, spills).
+// (Spills: 68 bytes at D = 128, 84 at 64.)
 // Every mbarrier wait is bounded (clock budget); a timeout sets ETIMEOUT and
 // the CTA drains and returns.
 #include <cuda.h>

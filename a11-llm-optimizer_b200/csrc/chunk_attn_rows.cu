@@ -28,7 +28,10 @@
 // Tokens past the last visible one are never read: their copies are zero-filled.
 // Measured (one B200): 32 sequences of one token over up to 4096 (32 / 4 heads of
 // 128, 200 MB) 41 us = 4.9 TB/s, 61 through chunk_attn_tc; one token over 32767
-// (67 MB, 37 pieces per KV head) 23.7 us, 33 through chunk_attn_tc with 64 splits.
+// (67 MB, 37 pieces per KV head) 23.8 us, 33 through chunk_attn_tc with 64 splits; with
+// 24 / 8 heads of 64, 32 sequences 43.5 us = 4.6 TB/s, one token over 32767 23.7 us. The
+// kernel of 25 to 32 rows of 128 dims spills 160 bytes.
+// The probabilities are rounded to bf16 for the product with V, as in chunk_attn.cu.
 #include <algorithm>
 
 #include "common.cuh"

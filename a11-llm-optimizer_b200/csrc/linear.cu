@@ -12,15 +12,16 @@
 //
 // Three kernels, chosen in launch_linear by a cost model of their tiles:
 //   linear_skinny (linear_skinny.cu)  up to 32 rows: HBM-bound weight streaming
-//   linear_tile   128 rows x 64 or 128 weight rows a CTA, K split over the CTAs
+//   linear_tile   128 rows x 32, 64 or 128 weight rows a CTA, K split over the CTAs
 //                 of a cluster (1 to 8): sizes whose tiles alone would leave most
 //                 SMs idle. The partial sums meet in distributed shared memory,
 //                 added in rank order.
 //   linear_pair   persistent CTA pairs (cta_group::2), 256 x 256 tiles: sizes
 //                 that fill the GPU. Tensor-bound; structure as in lm_head.cu.
-// Measured (one B200): 2048 x 8192 -> 2048 60 us = 1.14 PFLOP/s (64 tiles on 74
-// pairs), 8192 x 2048 -> 8192 gated e4m3 237 to 242 us = 2.3 PFLOP/s (10.4 TB/s of operands
-// from L2 into the SMs), 197 x 1000 -> 1531 9.4 us, 64 x 8192 -> 2048 14.5 us.
+// Measured (one B200): 2048 x 8192 -> 2048 with a residual 60 us = 1.14 PFLOP/s (64 tiles on
+// 74 pairs), 8192 x 2048 -> 8192 gated e4m3 237 to 242 us = 2.3 PFLOP/s (2.15 GB of operands
+// from L2 into the SMs, 9 TB/s; 10.6 in a cold launch of 203 us), 197 x 1000 -> 1531 9.4 us,
+// 64 x 8192 -> 2048 bf16 13.0 us, e4m3 9.6.
 // A gated product takes gate and weight rows side by side in one tile (half the
 // columns each), so x is staged once for both and act(u) v is formed from two
 // column ranges of one accumulator: the 2 N intermediate is never written.
@@ -691,7 +692,8 @@ int tile_slots(int split, int sms) {
 // what a tile spends besides (filling the ring, exchanging sums, the epilogue).
 // Fitted to a sweep of every (BN, split) over 14 sizes of 48 to 2048 rows, K 512
 // to 8192 and N 200 to 8192; the choice was the fastest there or within 6 % of it.
-// For instance 64 x 8192 -> 2048: 64/4 14.2 us, 32/2 18.7, 64/1 33.6, pairs 43.9;
+// Eleven of them were bf16 and three e4m3; one set of constants serves both types,
+// gated or not. For instance 64 x 8192 -> 2048 with a residual: 64/4 14.2 us, 32/2 18.7, 64/1 33.6, pairs 43.9;
 // 768 x 4096 -> 4096: pairs 26.3, 128/2 45.5; 197 x 1000 -> 1531: 64/2 10.0, 32/1 10.4.
 struct Plan {
     int bn = kPairN, split = 1;

@@ -15,8 +15,10 @@
 // instructions.
 // e4m3 values are widened to f16 (exact) for the same instruction: products of
 // two e4m3 values are exact in fp32, as are all but the sums.
-// Measured (one B200): 1 x 2048 -> 2 x 8192 bf16 12.9 us = 5.2 TB/s (15.4 with 16-byte
-// loads and one column tile a block), 32 x 2048 -> 5120 e4m3 7.6 us.
+// Measured (one B200): 1 x 2048 -> 2 x 8192 bf16 12.6 us = 5.3 TB/s (15.4 with 16-byte
+// loads and one column tile a block), 32 x 2048 -> 5120 e4m3 7.6 us (9.1 where the
+// weights of every call come from HBM), 1 x 8192 -> 2048 bf16 10.1 us. Spills: 24 bytes in
+// the e4m3 gated kernel of 25 to 32 rows, 8 in the bf16 one of 9 to 16.
 #include <cuda_fp16.h>
 
 #include "epilogue.cuh"
@@ -195,7 +197,7 @@ cudaError_t launch_nt(const SkinnyParams &p, cudaStream_t s) {
     const int mt = kTwo && p.N >= 32 * 148 ? 2 : 1;
     const int blocks = (p.N + 16 * mt - 1) / (16 * mt);
     // 8 warps share K; 16 when the blocks do not fill the SMs and K has slices for
-    // them (1 x 8192 -> 2048: 10.3 us against 14.7)
+    // them (1 x 8192 -> 2048: 10.1 us against 14.7)
     const int warps = blocks < 148 && p.k_bytes >= 16 * 128 ? 16 : 8;
     const size_t smem = (size_t)warps * (GATED ? 2 : 1) * mt * NT * 128 * sizeof(float);
     auto go = [&](auto kernel) {

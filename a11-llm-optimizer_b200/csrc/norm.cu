@@ -23,7 +23,8 @@
 // on, and the up to 2 x 7 elements before and after it by one thread each.
 // Where the tensors differ in that distance, every access is one element.
 // Measured (one B200): 8190 x 4999 fp32 104 to 109 us = 6.0 to 6.3 TB/s (188 with one element per
-// access), 2048 x 2048 bf16 to e4m3 7.0 us, one row of 2048 2.6 us.
+// access), 2048 x 2048 bf16 to e4m3 6.9 to 7.0 us; one row of 2048 2.8 us,
+// which is the host's call. (Spills: 20 bytes in the fp32 kernel of unaligned rows above 8192 to e4m3.)
 #include <cuda_fp8.h>
 
 #include "common.cuh"

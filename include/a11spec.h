@@ -289,6 +289,8 @@ int a11s_tree_attention(const void *q, const void *k_pool, const void *v_pool, i
  * most 128 query heads per KV head. max_kv_len >= every ctx_lens[b] + n_new[b]
  * sizes the split of long caches (a smaller value costs speed, not results);
  * page_table holds at least that many positions.
+ * Scores, statistics, sums and accumulators are fp32; the probabilities are rounded
+ * to bf16 for the product with V, as in a11s_tree_attention.
  * Pool positions past ctx_lens[b] + n_new[b] - 1 never reach a result, whatever
  * they hold. A non-finite V row of a live token may reach the rows of earlier
  * tokens of its 128-key block (0 x Inf in the product).
@@ -317,7 +319,7 @@ int a11s_chunk_attention(const void *q, int64_t q_stride, const void *k_pool, co
  * sum (nullable): h rounded to `dtype`; it may be x or residual (in place). The
  *   norm is taken of the unrounded h.
  * out of the type out_dtype: `dtype`, or A11S_E4M3 with scales[row] =
- *   max(max|y| / 448, 2^-100) and out = y / scale, rounded to nearest even; then
+ *   max(max|y| / 448, 2^-100) and out = y / scale (the fp32 quotient), rounded to nearest even; then
  *   scales fp32 [rows] is required. out may not overlap an input or sum.
  * A row that holds a NaN or an infinity, or whose squares overflow fp32, gives
  * what these formulas give. 1 <= dim <= A11S_NORM_MAX_DIM. Rows and strides that
