@@ -41,7 +41,8 @@ def building(folder: str):
     file behind), with a scratch folder from which the result moves to its place whole."""
     lock = os.open(folder, os.O_RDONLY)
     try:
-        fcntl.flock(lock, fcntl.LOCK_EX)
+        with contextlib.suppress(OSError):  # no such locks there: several build, each in a folder of its own
+            fcntl.flock(lock, fcntl.LOCK_EX)
         with tempfile.TemporaryDirectory(prefix=".build-", dir=folder) as tmp:
             yield tmp
     finally:
@@ -147,7 +148,8 @@ def build_fast(force: bool = False) -> str:
         same_abi = out[:-len("-0123456789.so")]
         for old in glob.glob(glob.escape(same_abi) + "-*.so"):  # of earlier sources
             if old != out:
-                os.remove(old)
+                with contextlib.suppress(FileNotFoundError):
+                    os.remove(old)
     return out
 
 

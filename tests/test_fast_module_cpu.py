@@ -152,3 +152,15 @@ def test_processes_that_build_the_library_at_once(tmp_path):
         assert r.returncode == 0, err
     assert open(env["LOG"]).read() == "run\n"
     assert [f for f in os.listdir(os.path.join(path, "a11spec")) if f.startswith((".", "liba11"))] == ["liba11spec.so"]
+
+
+def test_a_folder_without_locks_still_builds(tmp_path):
+    """Some network file systems refuse a lock on a folder."""
+    path, env = _tree_with_compiler(tmp_path)
+    r = _python("""
+import fcntl
+def refuse(*a):
+    raise OSError(9, "Bad file descriptor")
+fcntl.flock = refuse
+""" + USE, path, **{k: v for k, v in env.items() if k != "PYTHONPATH"})
+    assert r.returncode == 0, r.stderr
